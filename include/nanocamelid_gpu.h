@@ -35,11 +35,13 @@ extern "C" {
 
 /* GGUF tensor type ids used by this path (gguf.rs:83-115). */
 #define NC_TYPE_F32 0
+#define NC_TYPE_F16 1
 #define NC_TYPE_Q4_0 2
 #define NC_TYPE_Q8_0 8
 #define NC_TYPE_Q4_K 12
 #define NC_TYPE_Q5_K 13
 #define NC_TYPE_Q6_K 14
+#define NC_TYPE_BF16 30
 
 typedef struct nc_ctx nc_ctx;         /* device context: device id, default stream */
 typedef struct nc_qmat nc_qmat;       /* device-resident repacked quantized matrix */
@@ -177,6 +179,85 @@ int nc_quantize_q8_0_batch(nc_ctx* ctx, const float* x, int8_t* x_i8, float* x_s
  * 8192. */
 int nc_rms_norm_q8_0_batch(nc_ctx* ctx, const float* x, const float* w, float eps, int8_t* x_i8, float* x_scales,
                            int batch_size, int64_t dim, void* stream);
+
+/* ---------------------------------------------------------------- paged key-value cache
+ * The attention half of a layer for several sequences at once, on the caller's device buffers (the
+ * reference serves one sequence: LlamaKvCache src/inference.rs:505-599, apply_rope :731-798,
+ * apply_attention_heads :4142-4172).  A prompt step rotates and appends its rows and attends over
+ * the packed prompts; a decode or verify step appends one or a few rows a sequence and attends over
+ * the pages.
+ *
+ * The cache is two pools of pages, [pages][page_size][kv_heads][head_dim] by the strides below (in
+ * elements, the same for both pools, head_dim contiguous; any order of the other three).  Position p
+ * of sequence s lies in page table[s][p / page_size] at p % page_size.  The element type is F32, F16
+ * or BF16, head_dim 64 or 128, page_size any.  Addresses are device addresses; pools and rows are
+ * 16-byte aligned with strides of whole 16 bytes, anything else is refused. */
+typedef struct nc_paged_kv {
+    uint64_t k_pages, v_pages; /* device addresses of the pools */
+    int64_t pages;
+    int64_t page_stride, pos_stride, head_stride; /* elements, at least head_dim */
+    int32_t elem_type;         /* NC_TYPE_F32, NC_TYPE_F16 or NC_TYPE_BF16 */
+    int32_t page_size, kv_heads, head_dim;
+} nc_paged_kv;
+
+/* The sequences of a step.  lens[s] counts the positions of sequence s with the step's new rows
+ * among them; its rows are row_start[s] .. row_start[s+1] of the packed rows (row_start 0: one row a
+ * sequence), and row i of n stands at position lens[s] - n + i.  The arrays are read by the kernels,
+ * so a captured graph follows what they hold at each replay.
+ *
+ * What they hold never makes a kernel leave the buffers.  A row of no position (lens[s] < n, as in a
+ * padded batch) is not appended and answers zeros; rows outside every sequence are left as they
+ * were; a row that needs a position past the table or max_len, or a page that is none of the pool's,
+ * is not appended and answers NaN.  Pages may be shared by sequences that only read them; two rows
+ * of one call that are appended to the same place leave either there. */
+typedef struct nc_paged_batch {
+    uint64_t table, lens, row_start; /* device int32 [seqs][table_stride], [seqs], [seqs + 1] or 0 */
+    int64_t table_stride;            /* entries between rows of the table, at least table_pages */
+    int32_t table_pages, seqs;
+    int32_t max_len;                 /* an upper bound of lens (it sizes launches and workspace), 0: the table's */
+    int32_t reserved;
+} nc_paged_batch;
+
+/* The (sin, cos) angles of positions 0 .. positions - 1 as the sessions compute theirs
+ * (cached_rope_angles src/inference.rs:860-901): out (host) [positions][rope_dim / 2][2] f32.
+ * factor 0: no Llama-3 frequency scaling, else the four llama.rope.scaling.* values.  Host only. */
+int nc_rope_table(int64_t positions, int32_t rope_dim, float freq_base, float factor, float original_context_length,
+                  float low_freq_factor, float high_freq_factor, float* out);
+/* Appends rows of k and v to the cache at their sequences' positions, k rotated on the way, and
+ * rotates q alongside.  k, v [rows][kv_heads * head_dim] and q [rows][heads * head_dim] of `type`
+ * (F32, F16 or BF16) with row strides in elements; q may be NULL.  Pairs (2j, 2j + 1), j <
+ * rope_dim / 2, turn by rope[position][j] (device f32, as nc_rope_table's), each product and sum
+ * rounded to f32 by itself as in the sessions; rope NULL: no rotation.  The cache gets each value
+ * rounded once to its type.  q_out and k_out (NULL: not wanted) receive the rotated rows,
+ * contiguous, of `type`; they may be q and k themselves where those are contiguous.  A row of no
+ * position is given back unrotated; one past rope_positions gives NaN in the rotated pairs and is
+ * not appended. */
+int nc_paged_kv_append(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch* batch, int type, int64_t rows,
+                       const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* k_out, const void* q,
+                       int64_t q_stride, int32_t heads, void* q_out, const float* rope, int64_t rope_positions,
+                       int32_t rope_dim, void* stream);
+/* out[t][h] = sum_j softmax_j(scale * q[t][h].k_j) v_j over the positions up to row t's own; query
+ * head h reads kv head h / (heads / kv_heads).  q [rows][heads * head_dim] of `type` with a row
+ * stride, out contiguous of `type`; type F32 or the cache's.  Any number of rows a sequence; meant
+ * for one (decode) to some (verify).  Scores, maxima and sums are f32; a row whose every score is
+ * -inf answers zeros.  A row's result depends on neither the batch nor the other rows of its
+ * sequence.  work: device scratch of nc_paged_attention_work_bytes (0: may be NULL), 16-byte
+ * aligned, used by this call alone until it has finished. */
+int64_t nc_paged_attention_work_bytes(const nc_paged_kv* kv, const nc_paged_batch* batch, int64_t rows, int32_t heads);
+int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch* batch, int type, int64_t rows,
+                       const void* q, int64_t q_stride, int32_t heads, float scale, void* out, void* work,
+                       int64_t work_bytes, void* stream);
+/* Causal attention over packed prompts: sequence s has query rows seq_start[s] .. seq_start[s+1] and
+ * key rows kv_start[s] .. kv_start[s+1] (device int32; kv_start NULL: the query rows'); row i of n
+ * sees the keys 0 .. m - n + i of m, so a prompt may continue one whose keys come first.  q [rows][
+ * heads * head_dim], k and v [kv_rows][kv_heads * head_dim] of `type` (F32, F16, BF16) with row
+ * strides in elements, 16-byte aligned; out contiguous of `type`.  Scores, maxima and sums are f32.
+ * A row that sees no key answers zeros, and so does one whose every score is -inf; rows outside
+ * every sequence are left as they were; starts outside the tensors count as their ends. */
+int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t kv_rows, const void* q, int64_t q_stride,
+                        const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t heads,
+                        int32_t kv_heads, int32_t head_dim, const int32_t* seq_start, const int32_t* kv_start,
+                        int32_t seqs, float scale, void* out, void* stream);
 
 /* ---------------------------------------------------------------- stochastic acceptance
  * No reference counterpart: the reference's temperature path matches sampled tokens

@@ -12,6 +12,9 @@ libnanocamelid_hip.so.  Names follow the reference:
 * ``Session.verify_greedy``      -- the k+1 verify of src/speculative.rs:122-286
 * ``generate_speculative_draft`` -- speculative_decoding_step, src/speculative.rs:299-494
 
+Operators for several sequences at once, which the reference has no counterpart of:
+``PagedKV`` / ``PagedBatch``, ``paged_kv_append``, ``paged_attention``, ``packed_attention``.
+
 Everything runs in the native library on the GPU; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -20,13 +23,15 @@ import ctypes as C
 
 import numpy as np
 
-from ._ffi import (NC_TYPE_Q4_0, NC_TYPE_Q4_K, NC_TYPE_Q5_K, NC_TYPE_Q6_K, NC_TYPE_Q8_0, DecodeStats, LoadOpts, ModelConfig, NcError, SynthSpec,
-                   VerifyResult, check, lib)
+from ._ffi import (NC_EINVAL, NC_TYPE_BF16, NC_TYPE_F16, NC_TYPE_F32, NC_TYPE_Q4_0, NC_TYPE_Q4_K, NC_TYPE_Q5_K, NC_TYPE_Q6_K,
+                   NC_TYPE_Q8_0, DecodeStats, LoadOpts, ModelConfig, NcError, PagedBatchView, PagedKVView, SynthSpec, VerifyResult,
+                   check, lib)
 
 __all__ = ["Context", "QMat", "Model", "Session", "matmul_quantized_batch", "matmul_blockdots",
            "quantize_f32_to_q8_0_batch", "synth_gguf", "uniform_prompt", "oracle_draft",
            "generate_speculative_draft", "NcError", "NC_TYPE_Q4_0", "NC_TYPE_Q4_K", "NC_TYPE_Q5_K", "NC_TYPE_Q8_0",
-           "SYNTH_CONFIGS"]
+           "SYNTH_CONFIGS", "PagedKV", "PagedBatch", "rope_table", "paged_kv_append", "paged_attention",
+           "packed_attention"]
 
 
 def _u32(a):
@@ -205,6 +210,201 @@ def rms_norm_q8_0_batch(ctx: Context, x, w, eps: float):
     check(lib().nc_rms_norm_q8_0_batch(ctx.h, x.data_ptr(), w.data_ptr(), float(eps), q.data_ptr(), s.data_ptr(), n,
                                        dim, _stream_of(x)))
     return q, s
+
+
+def rope_table(positions: int, rope_dim: int, freq_base: float = 500000.0, scaling=None) -> np.ndarray:
+    """The sessions' (sin, cos) angles of positions 0 .. positions - 1, [positions][rope_dim / 2][2] f32
+    (cached_rope_angles, src/inference.rs:860-901).  scaling: (factor, original_context_length,
+    low_freq_factor, high_freq_factor) of the Llama-3 frequency scaling, or None.  Needs no GPU."""
+    out = np.empty((positions, rope_dim // 2, 2), np.float32)
+    check(lib().nc_rope_table(positions, rope_dim, float(freq_base), *(float(x) for x in scaling or (0, 0, 0, 0)),
+                              out.ctypes.data))
+    return out
+
+
+_ELEMENT_TYPES = {}
+
+
+def _element_type(who, t):
+    if not _ELEMENT_TYPES:
+        import torch
+        _ELEMENT_TYPES.update({torch.float32: NC_TYPE_F32, torch.float16: NC_TYPE_F16, torch.bfloat16: NC_TYPE_BF16})
+    code = _ELEMENT_TYPES.get(t.dtype)
+    if code is None:
+        raise NcError(NC_EINVAL, f"{who}: type must be float32, float16 or bfloat16")
+    return code
+
+
+def _refuse(who, why):
+    raise NcError(NC_EINVAL, f"{who}: {why}")
+
+
+def _int32(who, name, t, dims, device):
+    if t.dim() != dims or t.device != device or not t.is_contiguous() and (dims == 1 or t.stride(1) != 1):
+        _refuse(who, f"{name} must be a {dims}-dimensional tensor of contiguous rows on the cache's device")
+    if str(t.dtype) != "torch.int32":
+        _refuse(who, f"{name} must be int32")
+    return t.data_ptr()
+
+
+def _rows(who, name, t, heads, head_dim, like, rows=None):
+    """Row stride of packed rows [rows][heads][head_dim] whose heads lie end to end."""
+    if t.dtype != like.dtype or t.device != like.device:
+        _refuse(who, f"{name} must have the type and device of the other rows")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != head_dim or heads is not None and shape[1] != heads or rows is not None and shape[0] != rows:
+        _refuse(who, f"{name} has shape {tuple(shape)}")
+    row, head, one = t.stride()
+    if (one != 1 and head_dim > 1) or (head != head_dim and shape[1] > 1):
+        _refuse(who, f"the heads of a row of {name} must lie end to end")
+    return row if shape[0] > 1 else shape[1] * head_dim
+
+
+def _output(who, name, out, like):
+    import torch
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+        _refuse(who, f"{name} must be contiguous, with the shape, type and device of its rows")
+    return out
+
+
+def _on(who, ctx, t):
+    if t.device.type != "cuda" or t.device.index != ctx.device:
+        _refuse(who, "tensors must be on the context's device")
+
+
+class PagedKV:
+    """Two pools of cache pages (nc_paged_kv) over the caller's tensors: k_pages and v_pages
+    [pages][page_size][kv_heads][head_dim] of float32, float16 or bfloat16, with any strides that leave
+    head_dim contiguous and are the same for both (so also slices and permuted views)."""
+
+    def __init__(self, k_pages, v_pages):
+        who = "PagedKV"
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+            _refuse(who, "the pools must be [pages][page_size][kv_heads][head_dim] with the same strides")
+        if k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
+            _refuse(who, "the pools must have one type and device")
+        if k_pages.stride(3) != 1:
+            _refuse(who, "head_dim must be contiguous")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        pages, size, heads, hd = k_pages.shape
+        # the stride of a dimension of one is never used: any valid value does
+        a, b, c = (s if n > 1 else hd for s, n in zip(k_pages.stride()[:3], (pages, size, heads)))
+        self.view = PagedKVView(k_pages.data_ptr(), v_pages.data_ptr(), pages, a, b, c, _element_type(who, k_pages), size,
+                                heads, hd)
+        self.ref = C.byref(self.view)
+        self.kv_heads, self.head_dim, self.device, self.dtype = heads, hd, k_pages.device, k_pages.dtype
+
+
+class PagedBatch:
+    """The sequences of a step (nc_paged_batch): int32 device tensors table [seqs][pages], lens [seqs]
+    (positions, the step's new rows among them) and row_start [seqs + 1] (None: one row a sequence).
+    max_len: an upper bound of lens, which keeps launches and workspace small under a wide table."""
+
+    def __init__(self, table, lens, row_start=None, max_len: int = 0):
+        who = "PagedBatch"
+        seqs = lens.shape[0] if lens.dim() == 1 else -1
+        if table.dim() != 2 or table.shape[0] != seqs or row_start is not None and tuple(row_start.shape) != (seqs + 1,):
+            _refuse(who, "table is [seqs][pages], lens [seqs] and row_start [seqs + 1]")
+        if not 0 <= max_len < 1 << 31:
+            _refuse(who, "max_len must be 0 or an int32 bound")
+        device = table.device
+        pages = table.shape[1]
+        self.view = PagedBatchView(_int32(who, "table", table, 2, device), _int32(who, "lens", lens, 1, device),
+                                   0 if row_start is None else _int32(who, "row_start", row_start, 1, device),
+                                   table.stride(0) if seqs > 1 else pages, pages, seqs, max_len, 0)
+        self.ref = C.byref(self.view)
+        self.table, self.lens, self.row_start, self.device = table, lens, row_start, device
+
+
+def paged_kv_append(ctx: Context, cache: PagedKV, batch: PagedBatch, k, v, rope=None, q=None, want_k: bool = False,
+                    q_out=None, k_out=None):
+    """Appends rows k and v [rows][kv_heads][head_dim] to the cache, each at its sequence's position, k
+    rotated by rope [positions][rope_dim / 2][2] (a device tensor of rope_table's; None: no rotation), and
+    rotates q [rows][heads][head_dim] alongside.  Rows may be views of a fused buffer: the heads of a row
+    lie end to end, rows are 16-byte aligned.  Returns (rotated q or None, rotated k or None); k comes back
+    where want_k or k_out asks for it.  q_out and k_out may be q and k themselves if those are contiguous."""
+    import torch
+    who = "paged_kv_append"
+    _on(who, ctx, k)
+    if cache.device != k.device or batch.device != k.device:
+        _refuse(who, "the cache, the sequences and the rows must be on one device")
+    code = _element_type(who, k)
+    hd, rows = cache.head_dim, k.shape[0]
+    ks = _rows(who, "k", k, cache.kv_heads, hd, k)
+    vs = _rows(who, "v", v, cache.kv_heads, hd, k, rows)
+    qs, heads, qp, qo = 0, 0, None, None
+    if q is not None:
+        qs = _rows(who, "q", q, None, hd, k, rows)
+        heads, qp = q.shape[1], q.data_ptr()
+        q_out = _output(who, "q_out", q_out, q)
+        qo = q_out.data_ptr()
+    if want_k or k_out is not None:
+        k_out = _output(who, "k_out", k_out, k)
+    rp, positions, dim = None, 0, 0
+    if rope is not None:
+        if rope.dim() != 3 or rope.shape[2] != 2 or rope.dtype != torch.float32 or rope.device != k.device or not rope.is_contiguous():
+            _refuse(who, "rope must be a contiguous float32 [positions][rope_dim / 2][2] tensor on the rows' device")
+        rp, positions, dim = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
+    check(lib().nc_paged_kv_append(ctx.h, cache.ref, batch.ref, code, rows, k.data_ptr(), ks, v.data_ptr(), vs,
+                                   None if k_out is None else k_out.data_ptr(), qp, qs, heads, qo, rp, positions, dim,
+                                   _stream_of(k)))
+    return (q_out if q is not None else None), k_out
+
+
+def paged_attention(ctx: Context, cache: PagedKV, batch: PagedBatch, q, scale: float | None = None, out=None):
+    """Attention of the newest rows q [rows][heads][head_dim] of each sequence over its pages, up to each
+    row's own position; query head h reads kv head h // (heads / kv_heads).  q is float32 or of the
+    cache's type; scale defaults to 1 / sqrt(head_dim).  Returns [rows][heads][head_dim] of q's type.  The
+    scratch comes from torch's allocator on the current stream, so calls on different streams, and captured
+    graphs, share none."""
+    import torch
+    who = "paged_attention"
+    _on(who, ctx, q)
+    if cache.device != q.device or batch.device != q.device:
+        _refuse(who, "the cache, the sequences and the rows must be on one device")
+    code = _element_type(who, q)
+    hd = cache.head_dim
+    qs = _rows(who, "q", q, None, hd, q)
+    rows, heads = q.shape[0], q.shape[1]
+    out = _output(who, "out", out, q)
+    need = lib().nc_paged_attention_work_bytes(cache.ref, batch.ref, rows, heads)
+    if need < 0:
+        check(int(need))
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    check(lib().nc_paged_attention(ctx.h, cache.ref, batch.ref, code, rows, q.data_ptr(), qs, heads,
+                                   hd ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                                   None if work is None else work.data_ptr(), need, _stream_of(q)))
+    return out
+
+
+def packed_attention(ctx: Context, q, k, v, seq_start, kv_start=None, scale: float | None = None, out=None):
+    """Causal attention over packed prompts: q [rows][heads][head_dim], k and v [kv_rows][kv_heads][head_dim]
+    of one type (float32, float16, bfloat16), sequence s being the rows seq_start[s] .. seq_start[s + 1] (int32
+    device tensor) and, where kv_start is given, the keys kv_start[s] .. kv_start[s + 1]: the last query row of
+    a sequence sees all of its keys, the one before all but the last, and so on.  Rows may be views of a fused
+    buffer.  Returns [rows][heads][head_dim]; rows outside every sequence are left as they were in out."""
+    who = "packed_attention"
+    _on(who, ctx, q)
+    code = _element_type(who, q)
+    if q.dim() != 3 or k.dim() != 3 or seq_start.dim() != 1 or seq_start.shape[0] < 1:
+        _refuse(who, "rows are [rows][heads][head_dim], starts [seqs + 1]")
+    hd, kv = q.shape[2], k.shape[1]
+    qs = _rows(who, "q", q, None, hd, q)
+    ks = _rows(who, "k", k, kv, hd, q)
+    vs = _rows(who, "v", v, kv, hd, q, k.shape[0])
+    starts = _int32(who, "seq_start", seq_start, 1, q.device)
+    kstarts = None
+    if kv_start is not None:
+        if kv_start.shape != seq_start.shape:
+            _refuse(who, "kv_start must have seq_start's shape")
+        kstarts = _int32(who, "kv_start", kv_start, 1, q.device)
+    out = _output(who, "out", out, q)
+    check(lib().nc_packed_attention(ctx.h, code, q.shape[0], k.shape[0], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                                    q.shape[1], kv, hd, starts, kstarts, seq_start.shape[0] - 1,
+                                    hd ** -0.5 if scale is None else float(scale), out.data_ptr(), _stream_of(q)))
+    return out
 
 
 def temperature_probs_batch(ctx: Context, logits, temp: float, out=None):

@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libnanocamelid_hip.so")
 
 NC_OK, NC_EINVAL, NC_ENOMEM, NC_EHIP, NC_EFORMAT, NC_ERANGE = 0, -1, -2, -3, -4, -5
 NC_TYPE_F32, NC_TYPE_Q4_0, NC_TYPE_Q8_0, NC_TYPE_Q4_K, NC_TYPE_Q5_K, NC_TYPE_Q6_K = 0, 2, 8, 12, 13, 14
+NC_TYPE_F16, NC_TYPE_BF16 = 1, 30
 NC_GEMM_KERNEL_AUTO, NC_GEMM_KERNEL_DOT4, NC_GEMM_KERNEL_MFMA = 0, 1, 2
 NC_ATTN_SEQUENTIAL, NC_ATTN_SPLIT = 0, 1
 NC_PASS_DIRECT, NC_PASS_GRAPH = 0, 1
@@ -47,6 +48,17 @@ class VerifyResult(C.Structure):
 class DecodeStats(C.Structure):
     _fields_ = [("steps", C.c_int64), ("drafted", C.c_int64), ("accepted", C.c_int64), ("emitted", C.c_int64),
                 ("decode_seconds", C.c_double), ("prefill_seconds", C.c_double)]
+
+
+class PagedKVView(C.Structure):
+    _fields_ = [("k_pages", C.c_uint64), ("v_pages", C.c_uint64), ("pages", C.c_int64), ("page_stride", C.c_int64),
+                ("pos_stride", C.c_int64), ("head_stride", C.c_int64), ("elem_type", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class PagedBatchView(C.Structure):
+    _fields_ = [("table", C.c_uint64), ("lens", C.c_uint64), ("row_start", C.c_uint64), ("table_stride", C.c_int64),
+                ("table_pages", C.c_int32), ("seqs", C.c_int32), ("max_len", C.c_int32), ("reserved", C.c_int32)]
 
 
 class SynthSpec(C.Structure):
@@ -83,6 +95,13 @@ SIGNATURES = {
     "nc_quantize_q8_0_batch": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, _i64, _vp]),
     "nc_rms_norm_q8_0_batch": (C.c_int, [_vp, _vp, _vp, C.c_float, _vp, _vp, C.c_int, _i64, _vp]),
     "nc_bench_matmul": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp]),
+    "nc_rope_table": (C.c_int, [_i64, _i32, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, _vp]),
+    "nc_paged_kv_append": (C.c_int, [_vp, _vp, _vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp,
+                                     _i64, _i32, _vp]),
+    "nc_paged_attention_work_bytes": (_i64, [_vp, _vp, _i64, _i32]),
+    "nc_paged_attention": (C.c_int, [_vp, _vp, _vp, _i32, _i64, _vp, _i64, _i32, C.c_float, _vp, _vp, _i64, _vp]),
+    "nc_packed_attention": (C.c_int, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp,
+                                      _i32, C.c_float, _vp, _vp]),
     "nc_temperature_probs_batch": (C.c_int, [_vp, _vp, _vp, _i32, _i64, C.c_float, _vp]),
     "nc_sample_logits_batch": (C.c_int, [_vp, _vp, _i32, _i64, C.c_float, C.POINTER(C.c_uint64), _vp, _u32p, _vp]),
     "nc_stochastic_accept": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _i64, C.c_uint64, _i64, _vp, _vp]),

@@ -25,6 +25,24 @@ int fail(int code, const std::string& msg);
             return ::nc::fail(NC_EHIP, std::string(#call) + ": " + hipGetErrorString(_e)); \
     } while (0)
 
+// Makes a device the calling thread's current one for a scope and gives the former one back.
+struct DeviceGuard {
+    int before = -1, rc = NC_OK;
+    explicit DeviceGuard(int device) {
+        int now = 0;
+        hipError_t e = hipGetDevice(&now);
+        if (e == hipSuccess && now != device) {
+            e = hipSetDevice(device);
+            if (e == hipSuccess) before = now;
+        }
+        if (e != hipSuccess) rc = fail(NC_EHIP, std::string("device selection: ") + hipGetErrorString(e));
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+};
+
 // ---------------------------------------------------------------- stage timing
 // While t_stage_ev1 is set (a session's stage timing), kernels launched through NC_LAUNCH are
 // dispatched with events stamped by the dispatch itself: t_stage_ev0 records the first such

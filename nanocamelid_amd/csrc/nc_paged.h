@@ -1,0 +1,136 @@
+// What the paged-cache operators (paged.hip, packed.hip) share: where a row stands, where a position
+// lies, and how values of the three element types are read and written.
+//
+// Everything that comes from device memory here (lengths, row starts, page numbers) is checked where
+// it is used, so that no value of it makes a kernel leave the tensors: a row outside every sequence is
+// left alone, a position outside the table or the pool is not read or written.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __HIP__
+#define NC_PAGED_HD __host__ __device__ __forceinline__
+#else
+#define NC_PAGED_HD inline
+#endif
+
+namespace nc {
+
+// n / d by a multiplication, for 0 <= n < 2^31 and 1 <= d < 2^31: q = (mulhi(n, magic) + n) >> shift with
+// shift = ceil(log2 d) and magic = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery 1994); the
+// sum stays below 2^32 as mulhi(n, magic) <= n < 2^31.
+struct PageDiv {
+    uint32_t magic = 0, shift = 0, size = 1;
+};
+NC_PAGED_HD PageDiv page_div(uint32_t d) {
+    PageDiv p;
+    p.size = d;
+    while ((1ull << p.shift) < d) p.shift++;
+    p.magic = (uint32_t)((((1ull << p.shift) - d) << 32) / d + 1);
+    return p;
+}
+NC_PAGED_HD uint32_t page_of(uint32_t n, const PageDiv& p) {
+    return ((uint32_t)(((uint64_t)n * p.magic) >> 32) + n) >> p.shift;
+}
+
+// The last positions that a sequence's length and its table let a row reach.
+struct PagedSeqs {
+    const int32_t* table = nullptr;      // [seqs][table_stride], table_pages of each row used
+    const int32_t* lens = nullptr;       // [seqs] positions, the new rows among them
+    const int32_t* row_start = nullptr;  // [seqs + 1], or null: one row a sequence
+    int64_t table_stride = 0;
+    int32_t table_pages = 0, seqs = 0;
+    int32_t cap = 0;  // positions that can be named: min(max_len, table_pages * page size)
+    int32_t rows = 0;
+};
+
+struct PagedPool {
+    int64_t page_stride = 0, pos_stride = 0, head_stride = 0;  // elements, of both pools
+    int32_t pages = 0;
+    PageDiv div;
+};
+
+// Rows [begin, begin + n) of sequence s, inside the tensor whatever row_start holds.
+NC_PAGED_HD void seq_rows(const int32_t* start, int s, int rows, int& begin, int& n) {
+    if (!start) {
+        begin = s;
+        n = s < rows ? 1 : 0;
+        return;
+    }
+    const int b = start[s], e = start[s + 1];
+    begin = b < 0 ? 0 : (b > rows ? rows : b);
+    const int end = e < 0 ? 0 : (e > rows ? rows : e);
+    n = end > begin ? end - begin : 0;
+}
+
+// Element offset of position p (0 <= p < cap) of a sequence in the pools, or -1 where its page is none.
+NC_PAGED_HD int64_t position_offset(const int32_t* table_row, const PagedPool& pool, int p) {
+    const uint32_t pg = page_of((uint32_t)p, pool.div);
+    const int32_t id = table_row[pg];
+    if ((uint32_t)id >= (uint32_t)pool.pages) return -1;
+    return (int64_t)id * pool.page_stride + (int64_t)(p - (int)(pg * pool.div.size)) * pool.pos_stride;
+}
+
+#ifdef __HIP__
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The sequence that row t (the same for every lane of the wave) belongs to, or -1: 64 starts at a time.
+__device__ __forceinline__ int seq_of_row(const int32_t* start, int seqs, int t) {
+    if (!start) return t < seqs ? t : -1;
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base <= seqs; base += 64) {
+        const int i = base + lane;
+        const bool le = i <= seqs && start[i] <= t;
+        const int c = __popcll(__ballot(le));
+        before += c;
+        if (c < 64) break;
+    }
+    const int s = before - 1;
+    return s >= 0 && s < seqs ? s : -1;
+}
+
+// Eight consecutive values, 16-byte aligned.
+__device__ __forceinline__ void load8(const float* p, float* v) {
+    const f32x4 a = ((const f32x4*)p)[0], b = ((const f32x4*)p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+}
+__device__ __forceinline__ void load8(const _Float16* p, float* v) {
+    const f16x8 a = *(const f16x8*)p;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+}
+__device__ __forceinline__ void load8(const __bf16* p, float* v) {
+    const bf16x8 a = *(const bf16x8*)p;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+}
+// One rounding to nearest even where the type is narrower than f32: the result's own type.
+__device__ __forceinline__ void store8(float* p, const float* v) {
+    ((f32x4*)p)[0] = f32x4{v[0], v[1], v[2], v[3]};
+    ((f32x4*)p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+}
+__device__ __forceinline__ void store8(_Float16* p, const float* v) {
+    f16x8 a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a[i] = (_Float16)v[i];
+    *(f16x8*)p = a;
+}
+__device__ __forceinline__ void store8(__bf16* p, const float* v) {
+    bf16x8 a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
+    *(bf16x8*)p = a;
+}
+
+#endif
+
+}  // namespace nc

@@ -1418,6 +1418,40 @@ static double now_s() {
 
 using namespace nc;
 
+// cached_rope_angles (inference.rs:860-901) of positions 0 .. positions - 1, from glibc on the host:
+// theta = base.powf(-(2i)/rope_dim), Llama-3 frequency scaling (inference.rs:875-893),
+// (sin, cos) = (pos*theta).sin_cos().  out [positions][rope_dim / 2][2].
+static void rope_angles(int64_t positions, int64_t rope_dim, float base, bool scaled, float factor, float orig, float low,
+                        float high, float* out) {
+    const int64_t half = rope_dim / 2;
+    static float (*volatile p_sinf)(float) = sinf;
+    static float (*volatile p_cosf)(float) = cosf;
+    static float (*volatile p_powf)(float, float) = powf;
+    std::vector<float> theta(half);
+    for (int64_t i = 0; i < half; i++) {
+        float th = p_powf(base, -((float)(i * 2)) / (float)rope_dim);
+        if (scaled) {
+            const float wavelength = (2.0f * 3.14159265358979323846f) / th;
+            const float low_wl = orig / low, high_wl = orig / high;
+            if (wavelength >= high_wl) {
+                if (wavelength > low_wl) {
+                    th = th / factor;
+                } else {
+                    const float smooth = (orig / wavelength - low) / (high - low);
+                    th = ((1.0f - smooth) * th / factor) + (smooth * th);
+                }
+            }
+        }
+        theta[i] = th;
+    }
+    for (int64_t pos = 0; pos < positions; pos++)
+        for (int64_t i = 0; i < half; i++) {
+            const float angle = (float)pos * theta[i];
+            out[(pos * half + i) * 2] = p_sinf(angle);
+            out[(pos * half + i) * 2 + 1] = p_cosf(angle);
+        }
+}
+
 // ================================================================ C ABI
 extern "C" {
 
@@ -1700,6 +1734,17 @@ int nc_rms_norm_q8_0_batch(nc_ctx* ctx, const float* x, const float* w, float ep
                              stream ? (hipStream_t)stream : ctx->stream);
 }
 
+int nc_rope_table(int64_t positions, int32_t rope_dim, float freq_base, float factor, float original_context_length,
+                  float low_freq_factor, float high_freq_factor, float* out) {
+    if (!out || positions < 0 || positions > (1ll << 31) || rope_dim < 2 || rope_dim > 8192 || rope_dim % 2 ||
+        !(freq_base > 0.0f) ||
+        !(factor >= 0.0f))
+        return fail(NC_EINVAL, "nc_rope_table: bad arguments");
+    rope_angles(positions, rope_dim, freq_base, factor != 0.0f, factor, original_context_length, low_freq_factor,
+                high_freq_factor, out);
+    return NC_OK;
+}
+
 int nc_temperature_probs_batch(nc_ctx* ctx, const float* logits, float* probs, int32_t rows, int64_t vocab, float temp,
                                void* stream) {
     if (!ctx || !logits || !probs || rows < 1 || vocab < 1 || vocab > INT32_MAX || !(temp > 0.0f))
@@ -1887,39 +1932,12 @@ int nc_session_create(nc_model* m, int64_t max_ctx, int32_t max_batch, nc_sessio
     NC_HIP(hipHostMalloc((void**)&s->h_preds, 64 * sizeof(uint32_t), hipHostMallocDefault));
     NC_HIP(hipHostMalloc((void**)&s->h_result, 16 * sizeof(int32_t), hipHostMallocDefault));
     NC_HIP(hipHostMalloc((void**)&s->h_pos, 16 * sizeof(int32_t), hipHostMallocDefault));
-    // RoPE (sin, cos) table, cached_rope_angles (inference.rs:860-901), from glibc on the
-    // host: theta = base.powf(-(2i)/rope_dim), Llama-3 frequency scaling when the model
-    // carries it (inference.rs:875-893), (sin, cos) = (pos*theta).sin_cos().
+    // RoPE (sin, cos) table, scaled where the model carries the Llama-3 frequency scaling
     const int64_t half = c.rope_dimension_count / 2;
     std::vector<float> tab((size_t)max_ctx * half * 2);
-    static float (*volatile p_sinf)(float) = sinf;
-    static float (*volatile p_cosf)(float) = cosf;
-    static float (*volatile p_powf)(float, float) = powf;
-    std::vector<float> theta(half);
-    for (int64_t i = 0; i < half; i++) {
-        float th = p_powf(c.rope_freq_base, -((float)(i * 2)) / (float)c.rope_dimension_count);
-        if (c.rope_scaling) {
-            const float factor = c.rope_scaling_factor, orig = c.rope_scaling_original_context_length;
-            const float low = c.rope_scaling_low_freq_factor, high = c.rope_scaling_high_freq_factor;
-            const float wavelength = (2.0f * 3.14159265358979323846f) / th;
-            const float low_wl = orig / low, high_wl = orig / high;
-            if (wavelength >= high_wl) {
-                if (wavelength > low_wl) {
-                    th = th / factor;
-                } else {
-                    const float smooth = (orig / wavelength - low) / (high - low);
-                    th = ((1.0f - smooth) * th / factor) + (smooth * th);
-                }
-            }
-        }
-        theta[i] = th;
-    }
-    for (int64_t pos = 0; pos < max_ctx; pos++)
-        for (int64_t i = 0; i < half; i++) {
-            const float angle = (float)pos * theta[i];
-            tab[(pos * half + i) * 2] = p_sinf(angle);
-            tab[(pos * half + i) * 2 + 1] = p_cosf(angle);
-        }
+    rope_angles(max_ctx, half * 2, c.rope_freq_base, c.rope_scaling != 0, c.rope_scaling_factor,
+                c.rope_scaling_original_context_length, c.rope_scaling_low_freq_factor, c.rope_scaling_high_freq_factor,
+                tab.data());
     if ((rc = upload_f32(s->allocs, tab, &s->rope_tab))) return rc;
     s->ev.resize(4096);
     for (auto& e : s->ev) {
