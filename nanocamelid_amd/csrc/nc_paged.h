@@ -131,6 +131,44 @@ __device__ __forceinline__ void store8(__bf16* p, const float* v) {
     *(bf16x8*)p = a;
 }
 
+
+// ---------------------------------------------------------------- f32 values on 16-bit matrix products
+// A 16-bit product of f32 values: the value as a sum of 16-bit parts, each the rest rounded to nearest, so that
+// the products of the parts, exact and summed in f32, have f32's accuracy.  Three bf16 parts hold 24 bits at
+// any exponent; two f16 parts hold 22 of a value scaled into f16's range.
+template <typename T, int N>
+__device__ __forceinline__ void split_parts(float x, T (&part)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        part[i] = (T)x;
+        // the rest of an infinity is nothing, not NaN
+        x = __builtin_isinf((float)part[i]) ? 0.f : x - (float)part[i];
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<_Float16> {
+    using type = f16x8;
+};
+template <>
+struct Vec8<__bf16> {
+    using type = bf16x8;
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+// A maximum as the base of a row's exponents: 0 where nothing was seen, so that exp2(-inf - base) is 0.
+__device__ __forceinline__ float exp_base(float m) { return m == -__builtin_inff() ? 0.f : m; }
+
 #endif
 
 }  // namespace nc
