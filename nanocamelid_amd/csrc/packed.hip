@@ -3,6 +3,9 @@
 // rows sees its keys 0 .. m - n + i.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "nc_internal.h"
 #include "nc_paged.h"
 
@@ -17,57 +20,329 @@ struct PackedParams {
     float scale;
 };
 
-// One wave per (row, head): 64 keys at a time, a key a lane for the scores, a running maximum and sum, then
-// the values with head_dim over the lanes.
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kPackedRows = 128;  // query rows of a workgroup, 32 a wave
+
+// Four keys' values of one dimension: the 16 lanes of a group read four rows of 16 dimensions, eight bytes each,
+// and get a column back.
+template <typename V4>
+__device__ __forceinline__ V4 read_columns(const void* p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    auto q = (__attribute__((address_space(3))) s16x4*)(p);
+    return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q));
+}
+
+// Attention of 128 query rows of one head over their sequence's keys, a tile of keys at a time with a running
+// maximum and sum.
+//
+// Bound by the matrix products (4 head_dim operations a row and key) and, close behind, by the vector work of
+// the softmax.  Everything is transposed: scores^T = K q^T leaves a lane 16 scores of its own row for every 32
+// keys, and out^T = V^T p^T takes its weights from just there if its inner index counts the keys in that order,
+// so weights never cross lanes.  Keys and values go through LDS, shared by the four waves; rows of 16-byte pieces
+// whose order is turned by the row, so that the reads of both products are free of bank conflicts.  The next
+// tile's loads are in flight during a tile's products.
+//   16 bits: values are read as columns by the transposing LDS read, weights are rounded to the operands' type
+//   (as much as the answer's own rounding).
+//   f32: keys, values, queries and weights as three bf16 parts (nc_paged.h), of whose products the six largest
+//   are kept: what is left out is below 2^-24 of |q||k|.  The f32 products of the matrix cores run at a sixteenth
+//   of the bf16 rate, these at a sixth.
 template <typename A, int HD>
-__global__ __launch_bounds__(64) void packed_attention_kernel(PackedParams a) {
-    __shared__ float qs[HD];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int s = seq_of_row(a.seq_start, a.seqs, t);
-    if (s < 0) return;
-    int begin, n, kbegin, m;
-    seq_rows(a.seq_start, s, a.rows, begin, n);
-    seq_rows(a.kv_start, s, a.kv_rows, kbegin, m);
-    const int i = t - begin;
-    if (i < 0 || i >= n) return;
-    const A* q = (const A*)a.q + (int64_t)t * a.q_stride + h * HD;
-    for (int d = lane; d < HD; d += 64) qs[d] = (float)q[d] * a.scale;
-    __syncthreads();
-    const int seen = m - n + i + 1;
-    const int head = (h / (a.heads / a.kv_heads)) * HD;
-    const A* kb = (const A*)a.k + (int64_t)kbegin * a.k_stride + head;
-    const A* vb = (const A*)a.v + (int64_t)kbegin * a.v_stride + head;
-    float top = -__builtin_inff(), l = 0.f, acc[HD / 64] = {};
-    for (int base = 0; base < seen; base += 64) {
-        const int p = base + lane;
-        float score = -__builtin_inff();
-        if (p < seen) {
-            score = 0.f;
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load8(kb + p * a.k_stride + d, x);
-                for (int j = 0; j < 8; j++) score += qs[d + j] * x[j];
+__global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a, int64_t units) {
+    constexpr bool F32 = sizeof(A) == 4;
+    using E = std::conditional_t<F32, __bf16, A>;
+    using V8 = typename Vec8<E>::type;
+    typedef E V4 __attribute__((ext_vector_type(4)));
+    constexpr int NP = F32 ? 3 : 1;        // parts of a value
+    constexpr int BN = F32 ? 32 : 64;      // keys of a tile
+    constexpr int NB = F32 ? 1 : 2;        // LDS buffers
+    constexpr int PC = HD / 8;             // 16-byte pieces of an LDS row
+    constexpr int NL = BN * PC / 256;      // pieces of a tile that a thread moves
+    constexpr int KB = BN / 32, DT = HD / 32, KK = HD / 16;
+    __shared__ __attribute__((aligned(16))) E s_k[NB][NP][BN][HD], s_v[NB][NP][BN][HD];
+    __shared__ int s_odd[NB][2];  // the tile (from 1) whose keys, values held an infinity or NaN
+
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, h = lane >> 5;
+    const int G = a.heads / a.kv_heads;
+    const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : a.scale;
+    const float c = a.scale == 0.f ? 1.f : __builtin_fabsf(a.scale) * kLog2e;  // scores to base 2, positive
+
+    for (int64_t b = blockIdx.x; b < units; b += gridDim.x) {
+        // the kv heads first, so that one head's workgroups share an XCD's L2
+        const int kvh = (int)(b % a.kv_heads), head = kvh * G + (int)(b / a.kv_heads % G);
+        int64_t tile = b / a.heads;
+        // its sequence: tiles of 64 sequences at a time; a sequence's last rows, which see the most, first
+        int s = -1, q0 = 0, begin = 0, n = 0;
+        for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+            int mb = 0, mn = 0;
+            if (s0 + lane < a.seqs) seq_rows(a.seq_start, s0 + lane, a.rows, mb, mn);
+            const int mine = (mn + kPackedRows - 1) / kPackedRows;
+            int upto = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int x = __shfl_up(upto, d, 64);
+                if (lane >= d) upto += x;
+            }
+            const uint64_t past = __ballot(upto > tile);
+            if (past) {
+                const int at = __builtin_ctzll(past);
+                s = s0 + at;
+                begin = __shfl(mb, at, 64);
+                n = __shfl(mn, at, 64);
+                q0 = (int)(__shfl(upto, at, 64) - 1 - tile) * kPackedRows;
+                break;
+            }
+            tile -= __shfl(upto, 63, 64);
+        }
+        if (s < 0) return;  // past the last tile, and so is every later one
+        s = __builtin_amdgcn_readfirstlane(s);
+        q0 = __builtin_amdgcn_readfirstlane(q0);
+        begin = __builtin_amdgcn_readfirstlane(begin);
+        n = __builtin_amdgcn_readfirstlane(n);
+        int kbegin, m;
+        seq_rows(a.kv_start, s, a.kv_rows, kbegin, m);
+
+        // rows past the sequence's end take the last one's place and are not written
+        const int row = q0 + 32 * w + r < n ? q0 + 32 * w + r : n - 1;
+        const int before = m - n;  // may be negative
+        const int seen = before + row + 1;
+        const int wave_last = q0 + 32 * w + 31 < n ? q0 + 32 * w + 31 : n - 1;
+        const int wave_most = before + wave_last + 1;                           // keys that some row of the wave sees
+        const int wave_least = before + (q0 + 32 * w < n ? q0 + 32 * w : n - 1) + 1;  // that every row sees
+        const int last = q0 + kPackedRows - 1 < n ? q0 + kPackedRows - 1 : n - 1;
+        const int most = before + last + 1;
+        const int tiles = most > 0 ? (most + BN - 1) / BN : 0;
+        const A* q = (const A*)a.q + (int64_t)(begin + row) * a.q_stride + head * HD;
+        const A* kb = (const A*)a.k + (int64_t)kbegin * a.k_stride + kvh * HD;
+        const A* vb = (const A*)a.v + (int64_t)kbegin * a.v_stride + kvh * HD;
+
+        V8 qv[NP][KK];
+#pragma unroll
+        for (int d = 0; d < KK; d++) {
+            float x[8];
+            load8(q + 16 * d + 8 * h, x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                E part[NP];
+                split_parts(x[e] * sign, part);
+#pragma unroll
+                for (int p = 0; p < NP; p++) qv[p][d][e] = part[p];
             }
         }
-        float next = score;
-        for (int o = 32; o; o >>= 1) next = fmaxf(next, __shfl_xor(next, o, 64));
-        next = fmaxf(next, top);
-        const float base_of = next == -__builtin_inff() ? 0.f : next;
-        const float e = p < seen ? expf(score - base_of) : 0.f;
-        const float keep = expf(top - base_of);
-        float sum = e;
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        l = l * keep + sum;
-        top = next;
-        for (int c = 0; c < HD / 64; c++) acc[c] *= keep;
-        const int count = seen - base < 64 ? seen - base : 64;
-        for (int j = 0; j < count; j++) {
-            const float w = __shfl(e, j, 64);
-            for (int c = 0; c < HD / 64; c++) acc[c] += w * (float)vb[(base + j) * a.v_stride + c * 64 + lane];
+
+        // a thread's pieces of the next tile, as they lie in memory
+        typedef A Raw __attribute__((ext_vector_type(8)));
+        Raw kx[NL], vx[NL];
+        auto load_tile = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int id = tid + 256 * i, key = t * BN + id / PC;
+                const int64_t at = key < most ? key : most - 1;
+                kx[i] = *(const Raw*)(kb + at * a.k_stride + id % PC * 8);
+                vx[i] = *(const Raw*)(vb + at * a.v_stride + id % PC * 8);
+            }
+        };
+        auto store_tile = [&](int t) {
+            const int buf = NB == 2 ? t & 1 : 0;
+            // Values behind the last key or not finite are left out of the product (a zero weight times them would
+            // be no zero): f32 tiles are looked through as they are split, 16-bit ones where rows mask keys.
+            const bool edge = (t + 1) * BN > before + q0 + 1;
+            float kodd = 0.f, vodd = 0.f;  // NaN if there is one
+            if (F32 || edge) {
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        if (F32) kodd = __builtin_fmaf((float)kx[i][e], 0.f, kodd);
+                        vodd = __builtin_fmaf((float)vx[i][e], 0.f, vodd);
+                    }
+            }
+            if (F32 && kodd != kodd) s_odd[buf][0] = t + 1;
+            if (__ballot(vodd != vodd)) {
+                if (vodd != vodd) s_odd[buf][1] = t + 1;
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (!__builtin_isfinite((float)vx[i][e])) vx[i][e] = (A)0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int id = tid + 256 * i, key = id / PC, piece = id % PC;
+                const int pk = (piece ^ (key & (PC - 1))) * 8, pv = (piece ^ (2 * key & (PC - 1))) * 8;
+                if constexpr (F32) {
+                    V8 kp[3], vp[3];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        E part[3];
+                        split_parts(kx[i][e], part);
+#pragma unroll
+                        for (int p = 0; p < 3; p++) kp[p][e] = part[p];
+                        split_parts(vx[i][e], part);
+#pragma unroll
+                        for (int p = 0; p < 3; p++) vp[p][e] = part[p];
+                    }
+#pragma unroll
+                    for (int p = 0; p < 3; p++) {
+                        *(V8*)&s_k[buf][p][key][pk] = kp[p];
+                        *(V8*)&s_v[buf][p][key][pv] = vp[p];
+                    }
+                } else {
+                    *(Raw*)&s_k[buf][0][key][pk] = kx[i];
+                    *(Raw*)&s_v[buf][0][key][pv] = vx[i];
+                }
+            }
+        };
+
+        f32x16 o[DT] = {};
+        float top = -__builtin_inff(), l = 0.f;  // of the row; l of the lane's own keys
+        if (tid < 2 * NB) s_odd[tid / 2][tid % 2] = 0;
+        if (tiles > 0) load_tile(0);
+        __syncthreads();
+        if (NB == 2 && tiles > 0) {
+            store_tile(0);
+            if (tiles > 1) load_tile(1);
         }
+        for (int t = 0; t < tiles; t++) {
+            const int buf = NB == 2 ? t & 1 : 0;
+            if (NB == 1) {
+                store_tile(t);
+                if (t + 1 < tiles) load_tile(t + 1);
+            }
+            __syncthreads();
+            const int base = t * BN;
+            if (base < wave_most) {
+                f32x16 sc[KB] = {};
+#pragma unroll
+                for (int d = 0; d < KK; d++)
+#pragma unroll
+                    for (int j = 0; j < KB; j++) {
+                        const int key = 32 * j + r;
+                        V8 kv[NP];
+#pragma unroll
+                        for (int p = 0; p < NP; p++) kv[p] = *(const V8*)&s_k[buf][p][key][((2 * d + h) ^ (key & (PC - 1))) * 8];
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; p--)  // the smallest products first
+#pragma unroll
+                            for (int p2 = NP - 1 - p; p2 >= 0; p2--) sc[j] = mfma32(kv[p], qv[p2][d], sc[j]);
+                    }
+                if (F32 && s_odd[buf][0] == t + 1) {
+                    // keys that are not finite: parts of zero would make NaN of them, so their scores come from the
+                    // rows themselves
+#pragma unroll
+                    for (int j = 0; j < KB; j++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int key = base + 32 * j + 8 * (i / 4) + 4 * h + i % 4;
+                            float x = 0.f, odd = 0.f;
+                            if (key < seen)
+                                for (int d = 0; d < HD; d++) {
+                                    const float y = (float)kb[(int64_t)key * a.k_stride + d];
+                                    x += (float)q[d] * y;
+                                    odd = __builtin_fmaf(y, 0.f, odd);
+                                }
+                            if (odd != odd) sc[j][i] = x * sign;
+                        }
+                }
+                if (base + BN > wave_least) {
+#pragma unroll
+                    for (int j = 0; j < KB; j++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (base + 32 * j + 8 * (i / 4) + 4 * h + i % 4 >= seen) sc[j][i] = -__builtin_inff();
+                }
+                float next = top;
+#pragma unroll
+                for (int j = 0; j < KB; j++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) next = fmaxf(next, sc[j][i]);
+                next = fmaxf(next, __shfl_xor(next, 32, 64));
+                if (__ballot(next > top)) {
+                    const float keep = exp2_hw((top - exp_base(next)) * c);
+                    l *= keep;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[d] *= keep;
+                    top = next;
+                }
+                const float lift = exp_base(top) * c;
+#pragma unroll
+                for (int j = 0; j < KB; j++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        sc[j][i] = exp2_hw(__builtin_fmaf(sc[j][i], c, -lift));
+                        l += sc[j][i];
+                    }
+#pragma unroll
+                for (int j = 0; j < KB; j++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        V8 pv[NP];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            E part[NP];
+                            split_parts(sc[j][8 * u + e], part);
+#pragma unroll
+                            for (int p = 0; p < NP; p++) pv[p][e] = part[p];
+                        }
+                        const int i = lane & 15, key = 32 * j + 16 * u + 4 * h + i / 4;
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            const int piece = 4 * d + 2 * (lane >> 4 & 1) + (i >> 1 & 1);
+                            V8 vt[NP];
+#pragma unroll
+                            for (int p = 0; p < NP; p++) {
+                                const V4 lo = read_columns<V4>(&s_v[buf][p][key][(piece ^ (2 * key & (PC - 1))) * 8 + 4 * (i & 1)]);
+                                const V4 hi = read_columns<V4>(&s_v[buf][p][key + 8][(piece ^ (2 * (key + 8) & (PC - 1))) * 8 + 4 * (i & 1)]);
+                                vt[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                            }
+#pragma unroll
+                            for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                                for (int p2 = NP - 1 - p; p2 >= 0; p2--) o[d] = mfma32(vt[p], pv[p2], o[d]);
+                        }
+                    }
+                if (s_odd[buf][1] == t + 1) {
+                    // what was left out of the values, to the rows that see it
+                    for (int key = base; key < base + BN; key++)
+                        if (key < seen)
+#pragma unroll
+                            for (int d = 0; d < DT; d++)
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    const float x = (float)vb[(int64_t)key * a.v_stride + 32 * d + 8 * (i / 4) + 4 * h + i % 4];
+                                    if (!__builtin_isfinite(x)) o[d][i] += x;
+                                }
+                }
+            }
+            if (NB == 1) {
+                __syncthreads();
+            } else if (t + 1 < tiles) {
+                store_tile(t + 1);
+                if (t + 2 < tiles) load_tile(t + 2);
+            }
+        }
+        l += __shfl_xor(l, 32, 64);
+        if (q0 + 32 * w + r < n) {
+            const float inv = 1.f / l;
+            A* out = (A*)a.out + ((int64_t)(begin + row) * a.heads + head) * HD + 4 * h;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    typedef A Out __attribute__((ext_vector_type(4)));
+                    Out x;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = (A)(l == 0.f ? 0.f : F32 ? o[d][i + e] / l : o[d][i + e] * inv);
+                    *(Out*)(out + 32 * d + 2 * i) = x;
+                }
+        }
+        __syncthreads();
     }
-    A* out = (A*)a.out + ((int64_t)t * a.heads + h) * HD;
-    for (int c = 0; c < HD / 64; c++) out[c * 64 + lane] = (A)(l == 0.f ? 0.f : acc[c] / l);
 }
 
 }  // namespace nc
@@ -103,12 +378,14 @@ extern "C" int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t 
     DeviceGuard guard(ctx->device);
     if (guard.rc) return guard.rc;
     hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
-    const dim3 grid((unsigned)rows, heads);
+    // at most a tile more than its rows fill for every sequence; those past the last tile end at once
+    const int64_t units = (rows / kPackedRows + seqs) * heads;
+    const unsigned grid = (unsigned)std::min<int64_t>(units, 1 << 23);
     auto launch = [&]<typename A>() {
         if (head_dim == 64)
-            packed_attention_kernel<A, 64><<<grid, 64, 0, st>>>(a);
+            packed_attention_kernel<A, 64><<<grid, 256, 0, st>>>(a, units);
         else
-            packed_attention_kernel<A, 128><<<grid, 64, 0, st>>>(a);
+            packed_attention_kernel<A, 128><<<grid, 256, 0, st>>>(a, units);
         NC_HIP(hipGetLastError());
         return (int)NC_OK;
     };
