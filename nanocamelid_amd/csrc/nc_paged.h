@@ -63,16 +63,20 @@ NC_PAGED_HD void seq_rows(const int32_t* start, int s, int rows, int& begin, int
     n = end > begin ? end - begin : 0;
 }
 
-// Element offset of position p (0 <= p < cap) of a sequence in the pools, or -1 where its page is none.
-NC_PAGED_HD int64_t position_offset(const int32_t* table_row, const PagedPool& pool, int p) {
+// Element offset in the pools of position p of a sequence, in page id of the pool.
+NC_PAGED_HD int64_t place_in_page(int32_t id, int p, const PagedPool& pool) {
     const uint32_t pg = page_of((uint32_t)p, pool.div);
-    const int32_t id = table_row[pg];
-    if ((uint32_t)id >= (uint32_t)pool.pages) return -1;
     return (int64_t)id * pool.page_stride + (int64_t)(p - (int)(pg * pool.div.size)) * pool.pos_stride;
+}
+// The same by the sequence's row of the table (0 <= p < cap), or -1 where its page is none of the pool's.
+NC_PAGED_HD int64_t position_offset(const int32_t* table_row, const PagedPool& pool, int p) {
+    const int32_t id = table_row[page_of((uint32_t)p, pool.div)];
+    return (uint32_t)id < (uint32_t)pool.pages ? place_in_page(id, p, pool) : -1;
 }
 
 #ifdef __HIP__
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));

@@ -90,13 +90,14 @@ struct PagedAttnParams {
     int64_t q_stride;
     void* out;
     float *part_o, *part_ml;  // [row][head][slots][head_dim] and [2] (maximum, sum); null: slots is 1 or all in turn
-    int32_t heads, kv_heads, slots;
+    int64_t units;  // row groups of all sequences, or more
+    int32_t heads, kv_heads, slots, balanced;
     float scale;
 };
 
 // A sequence's positions in chunks of four waves, 32 KiB of keys and values a wave, or 16.
 template <typename C, int HD>
-constexpr int kWaveKeys = sizeof(C) == 4 && HD == 128 ? 32 : 64;
+constexpr int kWaveKeys = HD == 128 && sizeof(C) == 4 ? 32 : 64;
 template <typename C, int HD>
 constexpr int kChunkKeys = 4 * kWaveKeys<C, HD>;
 
@@ -108,9 +109,9 @@ struct RowSum {
     float m = -__builtin_inff(), l = 0.f, o[N] = {};
     __device__ __forceinline__ void add(float m2, float l2, float f, float g, const float* o2) {
         m = m2;
-        l = l * f + l2 * g;
+        l = __builtin_fmaf(l, f, l2 * g);
 #pragma unroll
-        for (int i = 0; i < N; i++) o[i] = o[i] * f + o2[i] * g;
+        for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(o[i], f, o2[i] * g);
     }
     __device__ __forceinline__ void add_chunk(float mc, float lc, const float* oc) {
         const float top = fmaxf(m, mc), base = exp_base(top);
@@ -118,6 +119,13 @@ struct RowSum {
     }
     __device__ __forceinline__ float answer(int i) const { return l == 0.f ? 0.f : o[i] / l; }
 };
+
+// A barrier that orders LDS alone, so that it does not wait for loads that are in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 // Attention of the rows of one sequence and kv head over chunks of its positions.
 //
@@ -132,7 +140,7 @@ struct RowSum {
 //   Weights of 16-bit rows are two parts as well: one alone would round as much as the answer's own rounding.
 //   f32: products of 16 x 16 x 4, whose operands need no turning.
 // A wave takes 32 or 64 positions at once: all their loads are in flight together, and one maximum serves them.
-template <typename A, typename C, int HD, int RT>
+template <typename A, typename C, int HD, int RT, bool ONE>
 __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(PagedAttnParams a) {
     constexpr bool F32 = sizeof(C) == 4;
     constexpr int KW = kWaveKeys<C, HD>, CH = 4 * KW, KT = KW / 16;
@@ -142,69 +150,235 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
     constexpr bool QSCALE = QP == 2;                           // f16 parts: the row scaled into f16's range
     // f16 weights carry 2^14, which keeps small ones normal numbers and cancels in the answer
     constexpr float PSHIFT = !F32 && !BF ? 14.f : 0.f;
+    // The next chunk's keys and values beside this one's, where the registers hold them; otherwise each half of the
+    // values takes the place of that half of the keys, and the next chunk's keys theirs.
+    constexpr bool EARLY = RT == 1 && (F32 || HD == 64 || ONE);
+    constexpr int JB = RT == 1 && QP < 3 && !ONE ? 2 : 1;  // LDS buffers of the waves' joining
     constexpr int OS = HD + 4;     // LDS row, skewed by four banks
     constexpr int ND = HD / 16;    // dimensions of a thread in the chunk's sum
-    __shared__ int64_t s_off[4][KW];
-    __shared__ float s_ml[4][RT][16][2];
-    __shared__ float s_o[4][RT][16][OS];
+    __shared__ int64_t s_off[2][4][KW];
+    using V8 = typename Vec8<std::conditional_t<F32, _Float16, C>>::type;
+    constexpr int QV = F32 ? HD / 16 : HD / 32;  // 16-byte pieces of a lane's queries, and of its key
+    __shared__ u32x4 s_q[RT][QP][QV][64];
+    __shared__ float s_factor[RT][16];
+    __shared__ int64_t s_scan[6];
+    __shared__ __attribute__((aligned(8))) float s_ml[JB][4][16][2];
+    __shared__ __attribute__((aligned(16))) float s_o[JB][4][16][OS];
 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int G = a.heads / a.kv_heads, groups = gridDim.y / a.kv_heads;
-    const int kvh = blockIdx.y % a.kv_heads;
-    const int64_t head_off = (int64_t)kvh * a.pool.head_stride;
-    const C* kb = (const C*)a.k_pages + head_off;
-    const C* vb = (const C*)a.v_pages + head_off;
+    const int G = a.heads / a.kv_heads;
+    const int32_t* row_start = a.seqs.row_start;
 
-    for (int s = blockIdx.z; s < a.seqs.seqs; s += gridDim.z) {
-        int begin, n;
-        seq_rows(a.seqs.row_start, s, a.seqs.rows, begin, n);
+    // Work comes as (row group, kv head, chunks from, to).  Either the grid names it: groups of all sequences one
+    // after the other along z, kv heads along y, chunks along x; or, where there are more chunks than workgroups fit
+    // the chip, all chunks of all sequences in one row are cut into equal parts, each of which kv_heads workgroups
+    // stream, a kv head each.  Those follow each other in the launch, as their heads do in the usual order of a
+    // pool: what lies together is read at one time.  The heads turn from part to part, so that no XCD (workgroups go
+    // to the eight in turn) reads one head only, whose rows may all lie in a few channels of its L2.
+    int64_t z = blockIdx.z, rest = 0, todo = 0;
+    int s = 0;
+    auto cost_of = [&](int i, int& begin, int& n, int& chunks) -> int64_t {
+        seq_rows(row_start, i, a.seqs.rows, begin, n);
+        const int len = a.seqs.lens[i], most = len < a.seqs.cap ? len : a.seqs.cap;
+        chunks = most > 0 ? (most - 1) / CH + 1 : 1;
+        return (int64_t)((n * G + 16 * RT - 1) / (16 * RT)) * chunks;
+    };
+    if (!ONE && a.balanced) {
+        // the sum over the sequences before the 256 at i0, of theirs up to the thread's own, and the thread's
+        int64_t all = 0, upto = 0, mine = 0;
+        auto scan = [&](int i0) {
+            int begin, n, chunks;
+            const int i = i0 + threadIdx.x;
+            mine = i < a.seqs.seqs ? cost_of(i, begin, n, chunks) : 0;
+            upto = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int64_t x = __shfl_up(upto, d, 64);
+                if (lane >= d) upto += x;
+            }
+            lds_barrier();
+            if (lane == 63) s_scan[w] = upto;
+            lds_barrier();
+            for (int i = 0; i < w; i++) upto += s_scan[i];
+            upto += all;
+            all += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+        };
+        for (int i0 = 0; i0 < a.seqs.seqs; i0 += 256) scan(i0);
+        const int64_t part = blockIdx.x / a.kv_heads, parts = gridDim.x / a.kv_heads;
+        const int64_t total = all, first = total * part / parts, past = total * (part + 1) / parts;
+        if (first == past) return;
+        todo = past - first;
+        auto claim = [&](int i0) {
+            if (upto - mine <= first && first < upto) s_scan[4] = i0 + threadIdx.x, s_scan[5] = first - (upto - mine);
+        };
+        if (a.seqs.seqs <= 256) {
+            claim(0);
+        } else {
+            all = 0;
+            for (int i0 = 0; i0 < a.seqs.seqs; i0 += 256) {
+                scan(i0);
+                claim(i0);
+            }
+        }
+        lds_barrier();
+        s = __builtin_amdgcn_readfirstlane((int)s_scan[4]);
+        rest = s_scan[5];
+    }
+
+    for (;;) {
+        int begin = 0, n = 0, r0 = 0, kvh = blockIdx.y, c = blockIdx.x, c_to = INT32_MAX;
+        if (!ONE && a.balanced) {
+            if (todo <= 0 || s >= a.seqs.seqs) return;
+            int chunks;
+            const int64_t cost = cost_of(s, begin, n, chunks);
+            if (rest >= cost) {
+                rest -= cost;
+                s++;
+                continue;
+            }
+            const int group = (int)(rest / chunks);
+            c = (int)(rest - (int64_t)group * chunks);
+            kvh = (blockIdx.x + blockIdx.x / a.kv_heads) % a.kv_heads;
+            r0 = group * (16 * RT);
+            const int take = (int)(todo < chunks - c ? todo : chunks - c);
+            c_to = c + take;
+            todo -= take;
+            rest += take;
+        } else if (!row_start) {
+            if (z >= a.units) return;
+            const int per = (G + 16 * RT - 1) / (16 * RT);
+            s = (int)(z / per);
+            r0 = (int)(z % per) * (16 * RT);
+            begin = s;
+            n = 1;
+            z += gridDim.z;
+        } else {
+            if (z >= a.units) return;
+            int64_t u = z;
+            s = -1;
+            for (int s0 = 0; s0 < a.seqs.seqs; s0 += 64) {
+                int mb = 0, mn = 0;
+                if (s0 + lane < a.seqs.seqs) seq_rows(row_start, s0 + lane, a.seqs.rows, mb, mn);
+                int upto = (mn * G + 16 * RT - 1) / (16 * RT);
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) {
+                    const int x = __shfl_up(upto, d, 64);
+                    if (lane >= d) upto += x;
+                }
+                const uint64_t past = __ballot(upto > u);
+                if (past) {
+                    const int at = __builtin_ctzll(past);
+                    s = s0 + at;
+                    begin = __builtin_amdgcn_readfirstlane(__shfl(mb, at, 64));
+                    n = __builtin_amdgcn_readfirstlane(__shfl(mn, at, 64));
+                    // counted from the sequence's last group
+                    r0 = __builtin_amdgcn_readfirstlane((int)(__shfl(upto, at, 64) - 1 - u)) * (16 * RT);
+                    break;
+                }
+                u -= __shfl(upto, 63, 64);
+            }
+            if (s < 0) return;  // past the last unit, and so is every later one
+            s = __builtin_amdgcn_readfirstlane(s);
+            z += gridDim.z;
+        }
+        const int step = a.balanced ? 1 : gridDim.x;
+        const int64_t head_off = (int64_t)kvh * a.pool.head_stride;
+        const C* kb = (const C*)a.k_pages + head_off;
+        const C* vb = (const C*)a.v_pages + head_off;
         const int32_t* table = a.seqs.table + s * a.seqs.table_stride;
         const int64_t before = (int64_t)a.seqs.lens[s] - n;  // positions before the first new row
-        const int64_t R = (int64_t)n * G;
-        for (int64_t r0 = (int64_t)(blockIdx.y / a.kv_heads) * (16 * RT); r0 < R; r0 += (int64_t)groups * (16 * RT)) {
+        const int R = n * G;  // below 2^31: so are all rows' heads
+        {
             // the positions that a row sees, at most cap of them
-            auto seen_of = [&](int64_t row) {
+            auto seen_of = [&](int row) {
                 const int64_t e = before + row / G + 1;
                 return (int)(e < 0 ? 0 : e > a.seqs.cap ? a.seqs.cap : e);
             };
-            const int64_t last = r0 + 16 * RT < R ? r0 + 16 * RT - 1 : R - 1;
+            const int last = R - r0 > 16 * RT ? r0 + 16 * RT - 1 : R - 1;
             const int least = seen_of(r0), most = seen_of(last);
-            const int chunks = most > 0 ? (most - 1) / CH + 1 : 1;
-            if ((int)blockIdx.x >= chunks) continue;
+            const int all_chunks = most > 0 ? (most - 1) / CH + 1 : 1, chunks = all_chunks < c_to ? all_chunks : c_to;
+            if (c >= chunks) continue;
 
-            // queries in operand order: row r of each tile, as many dimensions a lane as a product takes
-            int seen[RT];
-            float factor[RT];
-            constexpr int QN = F32 ? HD / 4 : 1, QV = F32 ? 1 : HD / 32;
-            float qf[RT][QN];
-            typename Vec8<std::conditional_t<F32, _Float16, C>>::type qv[RT][QP][QV];
+            // A wave's keys and values of a chunk.  Each is loaded as soon as the chunk before no longer needs its
+            // registers: keys when their scores are done, values when they are summed, so that loads are in flight
+            // through the softmax and the waves' joining.  They are issued whether or not there is a next chunk: behind
+            // a branch, every wait for an earlier load would have to wait for these as well.
+            typedef uint32_t VL __attribute__((ext_vector_type(F32 ? 4 : HD / 32)));  // 16 bytes, or HD / 16 values
+            constexpr int KV = QV, NV = F32 ? HD / 64 : 1;
+            u32x4 kx[KT][KV];
+            VL vx[KT][4][NV];
+            // Every lane finds one key's place, for its wave; -1: past the end, or its page is none of the pool's.  The
+            // page's number is asked for a chunk ahead, before that chunk's keys: loads return in order, and a later
+            // one would be waited for with all of those.
+            int32_t page_id = -1;
+            bool bad_pages = false;
+            auto ask = [&](int c) {
+                const int64_t p = (int64_t)c * CH + w * KW + lane;
+                page_id = lane < KW && p < a.seqs.cap ? table[page_of((uint32_t)p, a.pool.div)] : -1;
+            };
+            auto publish = [&](int buf, int c) {
+                const int p = c * CH + w * KW + lane;
+                const bool live = lane < KW && p < most, good = live && (uint32_t)page_id < (uint32_t)a.pool.pages;
+                if (lane < KW) s_off[buf][w][lane] = good ? place_in_page(page_id, p, a.pool) : -1;
+                bad_pages = __ballot(live && !good) != 0;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            };
+            // keys without a place read the pool's first row, which is there, and count as nothing
+            auto key_at = [&](int buf, int i) {
+                const int64_t at = s_off[buf][w][i];
+                return at < 0 ? (int64_t)0 : at;
+            };
+            auto load_keys = [&](int buf, int half) {
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                const int64_t row = r0 + 16 * t + r;
-                const bool live = row < R;
-                const int64_t rr = live ? row : r0;
-                seen[t] = live ? seen_of(row) : 0;
-                factor[t] = a.scale * kLog2e;
-                const A* q = (const A*)a.q + (begin + rr / G) * a.q_stride + (kvh * G + rr % G) * HD;
-                if constexpr (F32) {
+                for (int j = half * KT / 2; j < (half + 1) * KT / 2; j++) {
+                    const C* k = kb + key_at(buf, 16 * j + r) + (F32 ? 4 : 8) * g;
 #pragma unroll
-                    for (int j = 0; j < HD / 16; j++) {
-                        const f32x4 x = *(const f32x4*)(q + 16 * j + 4 * g);
+                    for (int d = 0; d < KV; d++) kx[j][d] = *(const u32x4*)(k + (F32 ? 16 : 32) * d);
+                    __builtin_amdgcn_sched_barrier(0);  // a few addresses at a time: they take two registers each
+                }
+            };
+            auto load_values = [&](int buf, int half) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) qf[t][4 * j + e] = x[e];
+                for (int j = half * KT / 2; j < (half + 1) * KT / 2; j++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const C* v = vb + key_at(buf, 16 * j + 4 * g + i) + (F32 ? 4 : ND) * r;
+#pragma unroll
+                        for (int h = 0; h < NV; h++) vx[j][i][h] = *(const VL*)(v + 64 * h);
                     }
-                } else if constexpr (QP == 1) {
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+
+            ask(c);
+            publish(0, c);
+            if (!ONE) ask(c + step);
 #pragma unroll
-                    for (int j = 0; j < QV; j++)
-                        qv[t][0][j] = *(const typename Vec8<C>::type*)(q + 32 * j + 8 * g);
+            for (int half = 0; half < 2; half++) load_keys(0, half);
+            if (EARLY) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) load_values(0, half);
+            }
+
+            // The queries in operand order, in LDS for the four waves: wave t has tile t's.  What scales a row's scores
+            // to base 2 goes beside them.
+            if (w < RT) {
+                const int row = r0 + 16 * w + r, rr = row < R ? row : r0;
+                const A* q = (const A*)a.q + (int64_t)(begin + rr / G) * a.q_stride + (kvh * G + rr % G) * HD;
+                float factor = a.scale * kLog2e;
+                if constexpr (F32 || QP == 1) {
+#pragma unroll
+                    for (int d = 0; d < QV; d++) s_q[w][0][d][lane] = *(const u32x4*)(q + (F32 ? 16 * d + 4 * g : 32 * d + 8 * g));
                 } else {
                     float x[QV][8];
                     float top = 0.f;
 #pragma unroll
-                    for (int j = 0; j < QV; j++) {
-                        load8(q + 32 * j + 8 * g, x[j]);
+                    for (int d = 0; d < QV; d++) {
+                        load8(q + 32 * d + 8 * g, x[d]);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[j][e]));
+                        for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[d][e]));
                     }
                     int shift = 0;
                     if (QSCALE) {  // the row's largest value to [2^9, 2^10)
@@ -212,196 +386,179 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                         top = fmaxf(top, __shfl_xor(top, 32, 64));
                         const int ex = (int)(__float_as_uint(top) >> 23);
                         shift = ex == 0 || ex == 255 ? 0 : 136 - ex;
-                        // applied in two steps: 2^shift alone may overflow, and so may its inverse
-                        factor[t] = __builtin_ldexpf(factor[t], -shift);
+                        factor = __builtin_ldexpf(factor, -shift);
                     }
 #pragma unroll
-                    for (int j = 0; j < QV; j++)
+                    for (int d = 0; d < QV; d++) {
+                        V8 parts[QP];
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             C part[QP];
-                            split_parts(QSCALE ? __builtin_ldexpf(x[j][e], shift) : x[j][e], part);
+                            split_parts(QSCALE ? __builtin_ldexpf(x[d][e], shift) : x[d][e], part);
 #pragma unroll
-                            for (int p = 0; p < QP; p++) qv[t][p][j][e] = part[p];
+                            for (int p = 0; p < QP; p++) parts[p][e] = part[p];
                         }
+#pragma unroll
+                        for (int p = 0; p < QP; p++) s_q[w][p][d][lane] = __builtin_bit_cast(u32x4, parts[p]);
+                    }
                 }
+                if (g == 0) s_factor[w][r] = factor;
             }
+            int seen[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++) seen[t] = r0 + 16 * t + r < R ? seen_of(r0 + 16 * t + r) : 0;
+            lds_barrier();
 
-            RowSum<ND> sum[RT];  // of row threadIdx.x / 16 and ND dimensions
-            for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+            // The thread's part in joining the waves: of each tile one row, ND dimensions.  Its output row, and its
+            // chunks (0: none, there is no such row).
+            const int row16 = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * ND;
+            RowSum<ND> sum[RT];
+            int unit[RT], own[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const int row = r0 + 16 * t + row16;
+                unit[t] = (begin + row / G) * a.heads + kvh * G + row % G;
+                own[t] = row >= R ? 0 : seen_of(row) > 0 ? (seen_of(row) - 1) / CH + 1 : 1;
+                // a row that needs a position past the last that can be named
+                if (before + row / G + 1 > a.seqs.cap) sum[t].l = __builtin_nanf("");
+            }
+            int buf = 0;
+            for (; c < chunks; c += step) {
                 const int base = c * CH + w * KW;
-                // every lane finds one key's place; those past the end and of bad pages read the pool's first
-                // row, which is there, and count as nothing
-                bool none = false;
-                if (lane < KW) {
-                    const int p = base + lane;
-                    int64_t at = p < most ? position_offset(table, a.pool, p) : -1;
-                    none = p < most && at < 0;
-                    s_off[w][lane] = at;
-                }
-                const bool masked = base + KW > least || __ballot(none) != 0;
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                // past the last chunk: no key has a place then
+                const int next = chunks - c > step ? c + step : INT32_MAX / CH;
+                const bool masked = base + KW > least || bad_pages;
 
                 f32x4 o[RT][ND] = {};
                 float m[RT], l[RT];
 #pragma unroll
                 for (int t = 0; t < RT; t++) m[t] = -__builtin_inff(), l[t] = 0.f;
-                if (base < most) {
+                {
                     f32x4 sc[RT][KT] = {};
-                    auto key_at = [&](int i) {
-                        const int64_t at = s_off[w][i];
-                        return at < 0 ? (int64_t)0 : at;
-                    };
-                    auto mask_scores = [&]() {
-                        if (!masked) return;
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+#pragma unroll
+                        for (int t = 0; t < RT; t++)
+#pragma unroll
+                            for (int d = 0; d < KV; d++) {
+                                u32x4 q[QP];
+#pragma unroll
+                                for (int p = 0; p < QP; p++) q[p] = s_q[t][p][d][lane];
+#pragma unroll
+                                for (int j = half * KT / 2; j < (half + 1) * KT / 2; j++) {
+                                    if constexpr (F32) {
+#pragma unroll
+                                        for (int e = 0; e < 4; e++)
+                                            sc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kx[j][d][e]), __uint_as_float(q[0][e]), sc[t][j], 0, 0, 0);
+                                    } else {
+#pragma unroll
+                                        for (int p = QP - 1; p >= 0; p--)
+                                            sc[t][j] = mfma16(__builtin_bit_cast(V8, kx[j][d]), __builtin_bit_cast(V8, q[p]), sc[t][j]);
+                                    }
+                                }
+                            }
+                        if (!EARLY) load_values(buf, half);
+                    }
+                    if (!ONE) {
+                        publish(buf ^ 1, next);
+                        ask(next + step);
+                    }
+                    if (!ONE && EARLY) {
+#pragma unroll
+                        for (int half = 0; half < 2; half++) load_keys(buf ^ 1, half);
+                    }
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        const float factor = s_factor[t][r];
+#pragma unroll
+                        for (int j = 0; j < KT; j++) sc[t][j] *= factor;
+                    }
+                    if (masked) {
 #pragma unroll
                         for (int j = 0; j < KT; j++)
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
                                 const int key = 16 * j + 4 * g + i;
-                                const bool bad = s_off[w][key] < 0;
+                                const bool bad = s_off[buf][w][key] < 0;
 #pragma unroll
                                 for (int t = 0; t < RT; t++)
                                     sc[t][j][i] = base + key < seen[t] ? (bad ? __builtin_nanf("") : sc[t][j][i])
                                                                        : -__builtin_inff();
                             }
-                    };
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                     // scores to weights, in base 2
-                    auto weigh = [&]() {
 #pragma unroll
-                        for (int t = 0; t < RT; t++) {
-                            float top = -__builtin_inff();
+                    for (int t = 0; t < RT; t++) {
+                        float top = -__builtin_inff();
 #pragma unroll
-                            for (int j = 0; j < KT; j++)
+                        for (int j = 0; j < KT; j++)
 #pragma unroll
-                                for (int i = 0; i < 4; i++) top = fmaxf(top, sc[t][j][i]);
-                            top = fmaxf(top, __shfl_xor(top, 16, 64));
-                            top = fmaxf(top, __shfl_xor(top, 32, 64));
-                            const float lift = exp_base(top) - PSHIFT;
-                            float total = 0.f;
-#pragma unroll
-                            for (int j = 0; j < KT; j++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const float e = exp2_hw(sc[t][j][i] - lift);
-                                    sc[t][j][i] = e;
-                                    total += e;
-                                }
-                            total += __shfl_xor(total, 16, 64);
-                            total += __shfl_xor(total, 32, 64);
-                            m[t] = top;
-                            l[t] = total;
-                        }
-                    };
-                    bool odd = false;  // an infinity or NaN among the values of a masked tile
-                    if constexpr (F32) {
-                        f32x4 kx[KT][HD / 16], vx[KT][4][HD / 64];
-#pragma unroll
-                        for (int j = 0; j < KT; j++) {
-                            const C* k = kb + key_at(16 * j + r) + 4 * g;
-#pragma unroll
-                            for (int d = 0; d < HD / 16; d++) kx[j][d] = *(const f32x4*)(k + 16 * d);
-                        }
+                            for (int i = 0; i < 4; i++) top = fmaxf(top, sc[t][j][i]);
+                        top = fmaxf(top, __shfl_xor(top, 16, 64));
+                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        const float lift = exp_base(top) - PSHIFT;
+                        float total = 0.f;
 #pragma unroll
                         for (int j = 0; j < KT; j++)
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                const C* v = vb + key_at(16 * j + 4 * g + i) + 4 * r;
-#pragma unroll
-                                for (int h = 0; h < HD / 64; h++) vx[j][i][h] = *(const f32x4*)(v + 64 * h);
+                                const float e = exp2_hw(sc[t][j][i] - lift);
+                                sc[t][j][i] = e;
+                                total += e;
                             }
+                        total += __shfl_xor(total, 16, 64);
+                        total += __shfl_xor(total, 32, 64);
+                        m[t] = top;
+                        l[t] = total;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    // A zero weight times an infinity is no zero: in masked tiles values that are not finite, and
+                    // those of keys without a place, are left out of the product.
+                    bool odd = false;
+                    if (masked) {
 #pragma unroll
                         for (int j = 0; j < KT; j++)
 #pragma unroll
-                            for (int d = 0; d < HD / 16; d++)
+                            for (int i = 0; i < 4; i++) {
+                                const bool gone = s_off[buf][w][16 * j + 4 * g + i] < 0;
 #pragma unroll
-                                for (int e = 0; e < 4; e++)
+                                for (int h = 0; h < NV; h++)
 #pragma unroll
-                                    for (int t = 0; t < RT; t++)
-                                        sc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[j][d][e], qf[t][4 * d + e], sc[t][j], 0, 0, 0);
-#pragma unroll
-                        for (int t = 0; t < RT; t++)
-#pragma unroll
-                            for (int j = 0; j < KT; j++) sc[t][j] *= factor[t];
-                        mask_scores();
-                        weigh();
-                        if (masked) {
-#pragma unroll
-                            for (int j = 0; j < KT; j++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const bool gone = s_off[w][16 * j + 4 * g + i] < 0;
-#pragma unroll
-                                    for (int h = 0; h < HD / 64; h++)
-#pragma unroll
-                                        for (int e = 0; e < 4; e++) {
-                                            const bool bad = !__builtin_isfinite(vx[j][i][h][e]);
+                                    for (int d = 0; d < (F32 ? 4 : HD / 32); d++) {
+                                        const uint32_t x = vx[j][i][h][d];
+                                        if constexpr (F32) {
+                                            const bool bad = (x & 0x7f800000u) == 0x7f800000u;
                                             odd |= bad && !gone;
-                                            if (bad || gone) vx[j][i][h][e] = 0.f;
+                                            vx[j][i][h][d] = bad || gone ? 0u : x;
+                                        } else {
+                                            constexpr uint32_t EXP = BF ? 0x7f80u : 0x7c00u;
+                                            const bool lo = (x & EXP) == EXP, hi = (x >> 16 & EXP) == EXP;
+                                            odd |= (lo || hi) && !gone;
+                                            vx[j][i][h][d] = gone ? 0u : (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
                                         }
-                                }
-                        }
+                                    }
+                            }
+                    }
+                    if constexpr (F32) {
 #pragma unroll
-                        for (int j = 0; j < KT; j++)
+                        for (int j = 0; j < KT; j++) {
+                            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                             for (int i = 0; i < 4; i++)
 #pragma unroll
-                                for (int h = 0; h < HD / 64; h++)
+                                for (int h = 0; h < NV; h++)
 #pragma unroll
                                     for (int e = 0; e < 4; e++)
 #pragma unroll
                                         for (int t = 0; t < RT; t++)
-                                            o[t][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[j][i][h][e], sc[t][j][i], o[t][4 * h + e], 0, 0, 0);
+                                            o[t][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vx[j][i][h][e]), sc[t][j][i], o[t][4 * h + e], 0, 0, 0);
+                            if (!ONE && !EARLY && j % (KT / 2) == KT / 2 - 1) load_keys(buf ^ 1, 2 * j / KT);
+                        }
                     } else {
-                        using V8 = typename Vec8<C>::type;
-                        typedef uint32_t VL __attribute__((ext_vector_type(HD / 32)));  // HD / 16 values
-                        V8 kx[KT][QV];
-                        VL vx[KT / 2][8];
-#pragma unroll
-                        for (int j = 0; j < KT; j++) {
-                            const C* k = kb + key_at(16 * j + r) + 8 * g;
-#pragma unroll
-                            for (int d = 0; d < QV; d++) kx[j][d] = *(const V8*)(k + 32 * d);
-                        }
-#pragma unroll
-                        for (int b = 0; b < KT / 2; b++)
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                vx[b][i] = *(const VL*)(vb + key_at(32 * b + 16 * (i / 4) + 4 * g + i % 4) + ND * r);
-#pragma unroll
-                        for (int j = 0; j < KT; j++)
-#pragma unroll
-                            for (int d = 0; d < QV; d++)
-#pragma unroll
-                                for (int t = 0; t < RT; t++)
-#pragma unroll
-                                    for (int p = QP - 1; p >= 0; p--) sc[t][j] = mfma16(kx[j][d], qv[t][p][d], sc[t][j]);
-#pragma unroll
-                        for (int t = 0; t < RT; t++)
-#pragma unroll
-                            for (int j = 0; j < KT; j++) sc[t][j] *= factor[t];
-                        mask_scores();
-                        weigh();
-                        if (masked) {
-                            constexpr uint32_t EXP = BF ? 0x7f80u : 0x7c00u;
-#pragma unroll
-                            for (int b = 0; b < KT / 2; b++)
-#pragma unroll
-                                for (int i = 0; i < 8; i++) {
-                                    const bool gone = s_off[w][32 * b + 16 * (i / 4) + 4 * g + i % 4] < 0;
-#pragma unroll
-                                    for (int d = 0; d < HD / 32; d++) {
-                                        const uint32_t x = vx[b][i][d];
-                                        const bool lo = (x & EXP) == EXP, hi = (x >> 16 & EXP) == EXP;
-                                        odd |= (lo || hi) && !gone;
-                                        vx[b][i][d] = gone ? 0u : (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
-                                    }
-                                }
-                        }
 #pragma unroll
                         for (int b = 0; b < KT / 2; b++) {
+                            __builtin_amdgcn_sched_barrier(0);
                             V8 pv[RT][PP];
 #pragma unroll
                             for (int t = 0; t < RT; t++)
@@ -417,7 +574,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                                 u32x4 x;  // dimension e of the lane's eight keys
 #pragma unroll
                                 for (int i = 0; i < 4; i++)
-                                    x[i] = __builtin_amdgcn_perm(vx[b][2 * i + 1][e / 2], vx[b][2 * i][e / 2],
+                                    x[i] = __builtin_amdgcn_perm(vx[2 * b + i / 2][2 * i % 4 + 1][0][e / 2], vx[2 * b + i / 2][2 * i % 4][0][e / 2],
                                                                  e % 2 ? 0x07060302u : 0x05040100u);
                                 const V8 vt = __builtin_bit_cast(V8, x);
 #pragma unroll
@@ -425,13 +582,14 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
 #pragma unroll
                                     for (int p = PP - 1; p >= 0; p--) o[t][e] = mfma16(vt, pv[t][p], o[t][e]);
                             }
+                            if (!ONE && !EARLY && b % (KT / 4) == KT / 4 - 1) load_keys(buf ^ 1, 4 * b / KT);
                         }
                     }
-                    // A zero weight times an infinity is no zero: in masked tiles such values were left out, and go
-                    // to the rows that see their key here.
+                    __builtin_amdgcn_sched_barrier(0);
+                    // the values left out go to the rows that see their key
                     if (__ballot(odd)) {
                         for (int key = 0; key < KW; key++) {
-                            const int64_t at = s_off[w][key];
+                            const int64_t at = s_off[buf][w][key];
                             if (at < 0) continue;
 #pragma unroll
                             for (int e = 0; e < ND; e++)
@@ -446,64 +604,62 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                                 }
                         }
                     }
-                }
-
-                // the four waves' sums to one, in their order
+                    if (!ONE && EARLY) {
 #pragma unroll
-                for (int t = 0; t < RT; t++)
-                    if (g == 0) s_ml[w][t][r][0] = m[t], s_ml[w][t][r][1] = l[t];
-                __syncthreads();
+                        for (int half = 0; half < 2; half++) load_values(buf ^ 1, half);
+                    }
+                }
+                buf ^= 1;
+
+                // The four waves' sums to one, in their order.  Two buffers in turn need one barrier: when a buffer is
+                // written again, all have passed the barrier of the other, behind their last reading of this one.
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    float top = s_ml[0][t][r][0];
+                    const int jb = JB == 2 ? buf : 0;
+                    if (r0 + 16 * t + r < R) {
+                        if (g == 0) *(f32x2*)s_ml[jb][w][r] = f32x2{m[t], l[t]};
 #pragma unroll
-                    for (int i = 1; i < 4; i++) top = fmaxf(top, s_ml[i][t][r][0]);
-                    const float f = exp2_hw(m[t] - exp_base(top));
+                        for (int e = 0; e < ND; e += 4)
 #pragma unroll
-                    for (int e = 0; e < ND; e += 4)
+                            for (int i = 0; i < 4; i++) {
+                                const int d = F32 ? 16 * e + 16 * g + 4 * i : ND * (4 * g + i) + e;
+                                *(f32x4*)&s_o[jb][w][r][d] = f32x4{o[t][e][i], o[t][e + 1][i], o[t][e + 2][i], o[t][e + 3][i]};
+                            }
+                    }
+                    lds_barrier();
+                    if (c < own[t]) {
+                        f32x2 ml[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) ml[i] = *(const f32x2*)s_ml[jb][i][row16];
+                        const float top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0])), lift = exp_base(top);
+                        float lc = 0.f, oc[ND] = {};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const int d = F32 ? 16 * e + 16 * g + 4 * i : ND * (4 * g + i) + e;
-                            *(f32x4*)&s_o[w][t][r][d] = f32x4{o[t][e][i], o[t][e + 1][i], o[t][e + 2][i], o[t][e + 3][i]} * f;
+                            const float f = exp2_hw(ml[i][0] - lift);
+                            lc = __builtin_fmaf(ml[i][1], f, lc);
+#pragma unroll
+                            for (int d = 0; d < ND; d++) oc[d] = __builtin_fmaf(s_o[jb][i][row16][d0 + d], f, oc[d]);
                         }
-                }
-                __syncthreads();
-                const int row16 = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * ND;
+                        if (a.slots > 1 && own[t] > 1) {
+                            const int64_t at = (int64_t)unit[t] * a.slots + c;
+                            if (d0 == 0) *(f32x2*)(a.part_ml + 2 * at) = f32x2{top, lc};
 #pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    float top = s_ml[0][t][row16][0];
+                            for (int d = 0; d < ND; d += 4)
+                                *(f32x4*)(a.part_o + at * HD + d0 + d) = f32x4{oc[d], oc[d + 1], oc[d + 2], oc[d + 3]};
+                        } else {
+                            sum[t].add_chunk(top, lc, oc);
+                            if (c == own[t] - 1) {
+                                A* out = (A*)a.out + (int64_t)unit[t] * HD + d0;
 #pragma unroll
-                    for (int i = 1; i < 4; i++) top = fmaxf(top, s_ml[i][t][row16][0]);
-                    const float lift = exp_base(top);
-                    float lc = 0.f, oc[ND] = {};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        lc += s_ml[i][t][row16][1] * exp2_hw(s_ml[i][t][row16][0] - lift);
-#pragma unroll
-                        for (int d = 0; d < ND; d++) oc[d] += s_o[i][t][row16][d0 + d];
-                    }
-                    const int64_t row = r0 + 16 * t + row16;
-                    if (row >= R) continue;
-                    const int64_t unit = (begin + row / G) * a.heads + kvh * G + row % G;
-                    const int mine = seen_of(row), own = mine > 0 ? (mine - 1) / CH + 1 : 1;
-                    if (c < own) sum[t].add_chunk(top, lc, oc);
-                    if (gridDim.x > 1 && own > 1) {
-                        if (c < own) {
-                            const int64_t at = unit * a.slots + c;
-                            a.part_ml[2 * at] = top;
-                            a.part_ml[2 * at + 1] = lc;
-#pragma unroll
-                            for (int d = 0; d < ND; d++) a.part_o[at * HD + d0 + d] = oc[d];
+                                for (int d = 0; d < ND; d++) out[d] = (A)sum[t].answer(d);
+                            }
                         }
-                    } else if (c == own - 1) {
-                        const bool past = before + row / G + 1 > a.seqs.cap;
-                        A* out = (A*)a.out + unit * HD + d0;
-#pragma unroll
-                        for (int d = 0; d < ND; d++) out[d] = (A)(past ? __builtin_nanf("") : sum[t].answer(d));
                     }
+                    if (JB == 1) lds_barrier();
                 }
-                __syncthreads();
+                if (ONE) break;
             }
+            lds_barrier();  // before the next unit's queries
         }
     }
 }
@@ -526,38 +682,43 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams a, int 
     const int seen = (int)(seen64 < 0 ? 0 : seen64 > a.seqs.cap ? a.seqs.cap : seen64);
     const int chunks = seen > 0 ? (seen - 1) / chunk + 1 : 1;
     if (chunks == 1) return;  // answered already
+    typedef float O __attribute__((ext_vector_type(ND)));
     const float* ml = a.part_ml + unit * a.slots * 2;
-    const float* o = a.part_o + unit * a.slots * HD + ND * lane;
+    const O* o = (const O*)(a.part_o + unit * a.slots * HD) + lane;
     RowSum<ND> sum;
+    if (seen64 > a.seqs.cap) sum.l = __builtin_nanf("");
     for (int c0 = 0; c0 < chunks; c0 += 64) {
         const int c = c0 + lane, count = chunks - c0 < 64 ? chunks - c0 : 64;
-        const float mc = c < chunks ? ml[2 * c] : -__builtin_inff(), lc = c < chunks ? ml[2 * c + 1] : 0.f;
-        float top = fmaxf(mc, sum.m);  // the largest score up to this chunk
+        O x[64];
+#pragma unroll
+        for (int i = 0; i < 64; i += 16)
+            if (i < count)
+#pragma unroll
+                for (int j = i; j < i + 16; j++) x[j] = o[(int64_t)(c0 + (j < count ? j : count - 1)) * (HD / ND)];
+        const f32x2 mine = c < chunks ? *(const f32x2*)(ml + 2 * c) : f32x2{-__builtin_inff(), 0.f};
+        float top = fmaxf(mine[0], sum.m);  // the largest score up to this chunk
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const float x = __shfl_up(top, d, 64);
-            if (lane >= d) top = fmaxf(top, x);
+            const float y = __shfl_up(top, d, 64);
+            if (lane >= d) top = fmaxf(top, y);
         }
         float prev = __shfl_up(top, 1, 64);
         if (lane == 0) prev = sum.m;
-        const float base = exp_base(top), f = exp2_hw(prev - base), g = exp2_hw(mc - base);
-        for (int i = 0; i < count; i += 8) {
-            float x[8][ND];
+        const float base = exp_base(top), f = exp2_hw(prev - base), g = exp2_hw(mine[0] - base);
+        auto of = [](float v, int at) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), at)); };
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int cc = i + j < count ? i + j : count - 1;
+        for (int j = 0; j < 64; j++)
+            if (j < count) {
+                float y[ND];
 #pragma unroll
-                for (int d = 0; d < ND; d++) x[j][d] = o[(int64_t)(c0 + cc) * HD + d];
+                for (int d = 0; d < ND; d++) y[d] = x[j][d];
+                sum.add(0.f, of(mine[1], j), of(f, j), of(g, j), y);
             }
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (i + j < count)
-                    sum.add(__shfl(top, i + j, 64), __shfl(lc, i + j, 64), __shfl(f, i + j, 64), __shfl(g, i + j, 64), x[j]);
-        }
+        sum.m = of(top, 63);
     }
     A* out = (A*)a.out + unit * HD + ND * lane;
 #pragma unroll
-    for (int d = 0; d < ND; d++) out[d] = (A)(seen64 > a.seqs.cap ? __builtin_nanf("") : sum.answer(d));
+    for (int d = 0; d < ND; d++) out[d] = (A)sum.answer(d);
 }
 
 namespace {
@@ -625,34 +786,38 @@ int with_types(int type, int cache, F f) {
     return f.template operator()<__bf16, __bf16, HD>();
 }
 
-// How a call is launched: tiles of 16 rows a workgroup, workgroups along the row groups of a sequence and along
-// its chunks, and chunk slots of a row's partial sums (1: none are kept).
+// How a call is launched: tiles of 16 rows a workgroup, units of such row groups, workgroups along a unit's chunks,
+// and chunk slots of a row's partial sums (1: none are kept).
 struct AttnPlan {
     int tiles = 1, chunk = 256, slots = 1, along = 1;
-    int64_t groups = 1;
+    bool balanced = false;
+    bool one = false;  // a workgroup has at most one chunk of a unit: nothing to load ahead
+    int64_t units = 1;
     int64_t bytes(int64_t rows, int heads, int hd) const { return slots > 1 ? rows * heads * slots * (hd + 2) * 4 : 0; }
 };
 
-int plan_attention(const nc_paged_kv& kv, const PagedSeqs& s, int heads, AttnPlan& p) {
-    const int64_t group = heads / kv.kv_heads;
-    p.chunk = kv.elem_type == NC_TYPE_F32 && kv.head_dim == 128 ? 128 : 256;
-    // rows of an average sequence, rounded up, decide the tiles: one where they fit one
-    const int64_t rows = s.seqs > 0 ? ((int64_t)s.rows + s.seqs - 1) / s.seqs * group : 1;
-    p.tiles = rows <= 16 ? 1 : 2;
-    // One sequence may hold nearly all rows: up to all row groups a sequence, as long as the launch stays within
-    // some 8192 workgroups or twice what the rows fill (those without rows end at once; the others loop).
-    const int64_t all = std::max<int64_t>(((int64_t)s.rows * group + 16 * p.tiles - 1) / (16 * p.tiles), 1);
-    const int64_t average = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
-    p.groups = !s.row_start ? average : std::min(all, std::max(2 * average, 8192 / ((int64_t)kv.kv_heads * std::max(s.seqs, 1)) + 1));
+AttnPlan plan_attention(const nc_paged_kv& kv, const PagedSeqs& s, int heads) {
+    AttnPlan p;
+    const int64_t group = heads / kv.kv_heads, seqs = std::max(s.seqs, 1);
+    p.chunk = kv.head_dim == 128 && kv.elem_type == NC_TYPE_F32 ? 128 : 256;
+    // Two tiles where sequences may have more than 16 rows (of the average, or twice that where they differ): one
+    // tile would read their keys and values twice.
+    const int64_t rows = ((int64_t)s.rows + seqs - 1) / seqs * group;
+    p.tiles = (s.row_start ? 2 * rows : rows) <= 16 ? 1 : 2;
+    const int64_t high = 16 * p.tiles;
+    p.units = s.row_start ? (int64_t)s.rows * group / high + seqs : seqs * ((group + high - 1) / high);
     const int64_t chunks = std::max<int64_t>(((int64_t)s.cap + p.chunk - 1) / p.chunk, 1);
-    // units of work without a split along the positions; from 8 a CU on the chip is full without one
-    const int64_t units = kv.kv_heads * std::max<int64_t>(s.seqs, all);
-    if (chunks > 1 && units < 2048) {
+    // From 8 units a CU on, the chip is full without a split along the positions, and two chunks are faster done in
+    // turn than joined.  Otherwise a workgroup takes a chunk, or where there may be more of them than fit the chip
+    // at once (two workgroups a CU, one with two tiles) an equal part of all.
+    const int64_t units = kv.kv_heads * p.units, fit = p.tiles == 1 ? 512 : 256;
+    if (chunks > 2 && units < 2048) {
         p.slots = (int)std::min<int64_t>(chunks, INT32_MAX);
-        p.along = (int)std::min<int64_t>(chunks, std::max<int64_t>(2, 16384 / units));
+        p.balanced = units * chunks > fit;
+        p.along = (int)(p.balanced ? std::max<int64_t>(fit / kv.kv_heads, 1) * kv.kv_heads : chunks);
     }
-    if (p.groups * kv.kv_heads > 65535) p.groups = std::max<int64_t>(1, 65535 / kv.kv_heads);
-    return NC_OK;
+    p.one = p.along == chunks && !p.balanced;
+    return p;
 }
 
 }  // namespace
@@ -715,8 +880,7 @@ extern "C" int64_t nc_paged_attention_work_bytes(const nc_paged_kv* kv, const nc
     if (int rc = read_cache("nc_paged_attention_work_bytes", kv, batch, rows, s, p)) return rc;
     if (heads < 1 || heads % kv->kv_heads || kv->kv_heads > 65535)
         return fail(NC_EINVAL, "nc_paged_attention_work_bytes: heads must be a multiple of the cache's heads, those at most 65535");
-    AttnPlan plan;
-    plan_attention(*kv, s, heads, plan);
+    const AttnPlan plan = plan_attention(*kv, s, heads);
     return plan.bytes(rows, heads, kv->head_dim);
 }
 
@@ -731,12 +895,13 @@ extern "C" int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_p
         return fail(NC_EINVAL, "nc_paged_attention: rows must be F32 or of the cache's type");
     if (heads < 1 || heads % kv->kv_heads || kv->kv_heads > 65535)
         return fail(NC_EINVAL, "nc_paged_attention: heads must be a multiple of the cache's heads, those at most 65535");
+    if (rows * heads > INT32_MAX - 512) return fail(NC_ERANGE, "nc_paged_attention: too many rows and heads");
     if (rows == 0 || batch->seqs == 0) return NC_OK;
     if (!q || !out) return fail(NC_EINVAL, "nc_paged_attention: null argument");
     if (bad_rows(q, q_stride, (int64_t)heads * kv->head_dim, size) || (uintptr_t)out % 16)
         return fail(NC_EINVAL, "nc_paged_attention: rows must be 16-byte aligned and not overlap");
-    AttnPlan plan;
-    plan_attention(*kv, a.seqs, heads, plan);
+    const AttnPlan plan = plan_attention(*kv, a.seqs, heads);
+    a.units = plan.units;
     const int64_t need = plan.bytes(rows, heads, kv->head_dim);
     if (need > 0 && (!work || (uintptr_t)work % 16 || work_bytes < need))
         return fail(NC_EINVAL, "nc_paged_attention: the workspace is missing, misaligned or too small");
@@ -752,17 +917,21 @@ extern "C" int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_p
     a.part_o = (float*)work;
     a.part_ml = (float*)work + (need > 0 ? rows * heads * plan.slots * kv->head_dim : 0);
     const int64_t joins = (rows * heads + 3) / 4;
-    if (need > 0 && joins > (1 << 24)) return fail(NC_ERANGE, "nc_paged_attention: too many rows and heads");
+    if (need > 0 && joins > (1 << 23)) return fail(NC_ERANGE, "nc_paged_attention: too many rows and heads");
     DeviceGuard guard(ctx->device);
     if (guard.rc) return guard.rc;
     hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
-    const dim3 grid((unsigned)plan.along, (unsigned)(plan.groups * kv->kv_heads), (unsigned)std::min(batch->seqs, 65535));
+    const dim3 grid((unsigned)plan.along, plan.balanced ? 1 : (unsigned)kv->kv_heads,
+                    plan.balanced ? 1 : (unsigned)std::min<int64_t>(plan.units, 65535));
+    a.balanced = plan.balanced;
     auto launch = [&]<typename A, typename C, int HD>() {
         if constexpr (std::is_same_v<A, float> || std::is_same_v<A, C>) {
-            if (plan.tiles == 1)
-                paged_attention_kernel<A, C, HD, 1><<<grid, 256, 0, st>>>(a);
+            if (plan.one)
+                plan.tiles == 1 ? paged_attention_kernel<A, C, HD, 1, true><<<grid, 256, 0, st>>>(a)
+                                : paged_attention_kernel<A, C, HD, 2, true><<<grid, 256, 0, st>>>(a);
             else
-                paged_attention_kernel<A, C, HD, 2><<<grid, 256, 0, st>>>(a);
+                plan.tiles == 1 ? paged_attention_kernel<A, C, HD, 1, false><<<grid, 256, 0, st>>>(a)
+                                : paged_attention_kernel<A, C, HD, 2, false><<<grid, 256, 0, st>>>(a);
             NC_HIP(hipGetLastError());
             if (plan.slots > 1) {
                 paged_join_kernel<A, HD><<<(unsigned)joins, 256, 0, st>>>(a, plan.chunk);
