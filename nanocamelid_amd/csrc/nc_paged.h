@@ -150,6 +150,16 @@ __device__ __forceinline__ void split_parts(float x, T (&part)[N]) {
     }
 }
 
+// The same of a value that is finite and within the type's range.
+template <typename T, int N>
+__device__ __forceinline__ void split_finite(float x, T (&part)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        part[i] = (T)x;
+        x -= (float)part[i];
+    }
+}
+
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -167,6 +177,13 @@ template <>
 struct Vec8<__bf16> {
     using type = bf16x8;
 };
+
+// The same value, of which the compiler does not know that: what rare branches compute from it stays in them,
+// instead of taking registers all along.
+__device__ __forceinline__ int kept_here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -29,6 +29,13 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 
 constexpr int kPackedRows = 128;  // query rows of a workgroup, 32 a wave
 
+// The power of two that takes the float of these bits to [2^9, 2^10): small parts of such values are normal f16
+// numbers, sums of their products far from infinite.
+__device__ __forceinline__ int shift_of(uint32_t bits) {
+    const int ex = (int)(bits >> 23) & 255;
+    return ex == 0 || ex == 255 ? 0 : 136 - ex;
+}
+
 // Four keys' values of one dimension: the 16 lanes of a group read four rows of 16 dimensions, eight bytes each,
 // and get a column back.
 template <typename V4>
@@ -49,23 +56,27 @@ __device__ __forceinline__ V4 read_columns(const void* p) {
 // tile's loads are in flight during a tile's products.
 //   16 bits: values are read as columns by the transposing LDS read, weights are rounded to the operands' type
 //   (as much as the answer's own rounding).
-//   f32: keys, values, queries and weights as three bf16 parts (nc_paged.h), of whose products the six largest
-//   are kept: what is left out is below 2^-24 of |q||k|.  The f32 products of the matrix cores run at a sixteenth
-//   of the bf16 rate, these at a sixth.
+//   f32: keys, values, queries and weights as two f16 parts (nc_paged.h), of whose products the smallest is left
+//   out, below 2^-24 of |q||k|.  Parts keep their bits for values down to 2^-16 of what they are scaled by: a row
+//   of queries by its largest, keys and values by the largest so far, which is a power of two that the scores'
+//   factor and the answer give back.  The f32 products of the matrix cores run at a sixteenth of the f16 rate,
+//   these at a third.
 template <typename A, int HD>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a, int64_t units) {
     constexpr bool F32 = sizeof(A) == 4;
-    using E = std::conditional_t<F32, __bf16, A>;
+    using E = std::conditional_t<F32, _Float16, A>;
     using V8 = typename Vec8<E>::type;
     typedef E V4 __attribute__((ext_vector_type(4)));
-    constexpr int NP = F32 ? 3 : 1;        // parts of a value
+    constexpr int NP = F32 ? 2 : 1;        // parts of a value
+    constexpr float PSHIFT = F32 ? 14.f : 0.f;  // keeps the parts of small weights normal numbers, cancels in the answer
     constexpr int BN = F32 ? 32 : 64;      // keys of a tile
     constexpr int NB = F32 ? 1 : 2;        // LDS buffers
     constexpr int PC = HD / 8;             // 16-byte pieces of an LDS row
     constexpr int NL = BN * PC / 256;      // pieces of a tile that a thread moves
     constexpr int KB = BN / 32, DT = HD / 32, KK = HD / 16;
     __shared__ __attribute__((aligned(16))) E s_k[NB][NP][BN][HD], s_v[NB][NP][BN][HD];
-    __shared__ int s_odd[NB][2];  // the tile (from 1) whose keys, values held an infinity or NaN
+    __shared__ int s_odd[2][2];           // by the tile's parity: the tile (from 1) whose keys, values held an infinity or NaN
+    __shared__ uint32_t s_top[4][2];      // f32: the largest of the next tile's keys, values that each wave moves
 
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, h = lane >> 5;
     const int G = a.heads / a.kv_heads;
@@ -122,16 +133,34 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
         const A* vb = (const A*)a.v + (int64_t)kbegin * a.v_stride + kvh * HD;
 
         V8 qv[NP][KK];
+        float factor = c;  // of the row's scores, to base 2
+        if constexpr (F32) {
+            float x[KK][8], top = 0.f;
 #pragma unroll
-        for (int d = 0; d < KK; d++) {
-            float x[8];
-            load8(q + 16 * d + 8 * h, x);
+            for (int d = 0; d < KK; d++) {
+                load8(q + 16 * d + 8 * h, x[d]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                E part[NP];
-                split_parts(x[e] * sign, part);
+                for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[d][e]));
+            }
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const int shift = shift_of(__float_as_uint(top));
+            factor = __builtin_ldexpf(c, -shift);
 #pragma unroll
-                for (int p = 0; p < NP; p++) qv[p][d][e] = part[p];
+            for (int d = 0; d < KK; d++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    E part[NP];
+                    split_parts(__builtin_ldexpf(x[d][e] * sign, shift), part);
+#pragma unroll
+                    for (int p = 0; p < NP; p++) qv[p][d][e] = part[p];
+                }
+        } else {
+#pragma unroll
+            for (int d = 0; d < KK; d++) {
+                float x[8];
+                load8(q + 16 * d + 8 * h, x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) qv[0][d][e] = (E)(x[e] * sign);
             }
         }
 
@@ -147,48 +176,83 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
                 vx[i] = *(const Raw*)(vb + at * a.v_stride + id % PC * 8);
             }
         };
-        auto store_tile = [&](int t) {
-            const int buf = NB == 2 ? t & 1 : 0;
-            // Values behind the last key or not finite are left out of the product (a zero weight times them would
-            // be no zero): f32 tiles are looked through as they are split, 16-bit ones where rows mask keys.
+        f32x16 o[DT] = {};
+        // f32: what keys and values are scaled by, 2^shift of the largest so far; no tile has asked yet
+        int kshift = 1000, vshift = 1000;
+        // Values behind the last key or not finite are left out of the product (a zero weight times them would be no
+        // zero): f32 tiles are looked through before they are split, 16-bit ones where rows mask keys.  f32: then the
+        // wave's largest key and value.
+        auto look_through = [&](int t) {
             const bool edge = (t + 1) * BN > before + q0 + 1;
+            if (!F32 && !edge) return;
             float kodd = 0.f, vodd = 0.f;  // NaN if there is one
-            if (F32 || edge) {
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (F32) kodd = __builtin_fmaf((float)kx[i][e], 0.f, kodd);
+                    vodd = __builtin_fmaf((float)vx[i][e], 0.f, vodd);
+                }
+            if (__ballot(kodd != kodd || vodd != vodd)) {
+                if (kodd != kodd) s_odd[t & 1][0] = t + 1;
+                if (vodd != vodd) s_odd[t & 1][1] = t + 1;
 #pragma unroll
                 for (int i = 0; i < NL; i++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        if (F32) kodd = __builtin_fmaf((float)kx[i][e], 0.f, kodd);
-                        vodd = __builtin_fmaf((float)vx[i][e], 0.f, vodd);
+                        if (F32 && !__builtin_isfinite((float)kx[i][e])) kx[i][e] = (A)0.f;
+                        if (!__builtin_isfinite((float)vx[i][e])) vx[i][e] = (A)0.f;
                     }
             }
-            if (F32 && kodd != kodd) s_odd[buf][0] = t + 1;
-            if (__ballot(vodd != vodd)) {
-                if (vodd != vodd) s_odd[buf][1] = t + 1;
+            if constexpr (F32) {
+                float kt = 0.f, vt = 0.f;
 #pragma unroll
                 for (int i = 0; i < NL; i++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (!__builtin_isfinite((float)vx[i][e])) vx[i][e] = (A)0.f;
+                    for (int e = 0; e < 8; e++) kt = fmaxf(kt, __builtin_fabsf(kx[i][e])), vt = fmaxf(vt, __builtin_fabsf(vx[i][e]));
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) kt = fmaxf(kt, __shfl_xor(kt, d, 64)), vt = fmaxf(vt, __shfl_xor(vt, d, 64));
+                if (lane == 0) s_top[w][0] = __float_as_uint(kt), s_top[w][1] = __float_as_uint(vt);
+            }
+        };
+        auto store_tile = [&](int t) {
+            const int buf = NB == 2 ? t & 1 : 0;
+            if constexpr (F32) {
+                uint32_t kt = 0, vt = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    kt = kt > s_top[i][0] ? kt : s_top[i][0];
+                    vt = vt > s_top[i][1] ? vt : s_top[i][1];
+                }
+                const int ks = shift_of(kt), vs = shift_of(vt);
+                kshift = ks < kshift ? ks : kshift;
+                if (vs < vshift) {
+                    if (vshift != 1000)
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[d][i] = __builtin_ldexpf(o[d][i], vs - vshift);
+                    vshift = vs;
+                }
             }
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int id = tid + 256 * i, key = id / PC, piece = id % PC;
                 const int pk = (piece ^ (key & (PC - 1))) * 8, pv = (piece ^ (2 * key & (PC - 1))) * 8;
                 if constexpr (F32) {
-                    V8 kp[3], vp[3];
+                    V8 kp[NP], vp[NP];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        E part[3];
-                        split_parts(kx[i][e], part);
+                        E part[NP];
+                        split_finite(__builtin_ldexpf(kx[i][e], kshift), part);
 #pragma unroll
-                        for (int p = 0; p < 3; p++) kp[p][e] = part[p];
-                        split_parts(vx[i][e], part);
+                        for (int p = 0; p < NP; p++) kp[p][e] = part[p];
+                        split_finite(__builtin_ldexpf(vx[i][e], vshift), part);
 #pragma unroll
-                        for (int p = 0; p < 3; p++) vp[p][e] = part[p];
+                        for (int p = 0; p < NP; p++) vp[p][e] = part[p];
                     }
 #pragma unroll
-                    for (int p = 0; p < 3; p++) {
+                    for (int p = 0; p < NP; p++) {
                         *(V8*)&s_k[buf][p][key][pk] = kp[p];
                         *(V8*)&s_v[buf][p][key][pv] = vp[p];
                     }
@@ -199,21 +263,18 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
             }
         };
 
-        f32x16 o[DT] = {};
         float top = -__builtin_inff(), l = 0.f;  // of the row; l of the lane's own keys
-        if (tid < 2 * NB) s_odd[tid / 2][tid % 2] = 0;
+        if (tid < 4) s_odd[tid / 2][tid % 2] = 0;
         if (tiles > 0) load_tile(0);
         __syncthreads();
-        if (NB == 2 && tiles > 0) {
+        if (tiles > 0) {
+            look_through(0);
+            if (F32) __syncthreads();
             store_tile(0);
             if (tiles > 1) load_tile(1);
         }
         for (int t = 0; t < tiles; t++) {
             const int buf = NB == 2 ? t & 1 : 0;
-            if (NB == 1) {
-                store_tile(t);
-                if (t + 1 < tiles) load_tile(t + 1);
-            }
             __syncthreads();
             const int base = t * BN;
             if (base < wave_most) {
@@ -231,16 +292,18 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
 #pragma unroll
                             for (int p2 = NP - 1 - p; p2 >= 0; p2--) sc[j] = mfma32(kv[p], qv[p2][d], sc[j]);
                     }
-                if (F32 && s_odd[buf][0] == t + 1) {
+                if (F32 && s_odd[t & 1][0] == t + 1) {
                     // keys that are not finite: parts of zero would make NaN of them, so their scores come from the
                     // rows themselves
+                    const int h4 = kept_here(4 * h);
 #pragma unroll
                     for (int j = 0; j < KB; j++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const int key = base + 32 * j + 8 * (i / 4) + 4 * h + i % 4;
+                            const int key = base + 32 * j + 8 * (i / 4) + h4 + i % 4;
                             float x = 0.f, odd = 0.f;
                             if (key < seen)
+#pragma unroll 1
                                 for (int d = 0; d < HD; d++) {
                                     const float y = (float)kb[(int64_t)key * a.k_stride + d];
                                     x += (float)q[d] * y;
@@ -256,25 +319,27 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
                         for (int i = 0; i < 16; i++)
                             if (base + 32 * j + 8 * (i / 4) + 4 * h + i % 4 >= seen) sc[j][i] = -__builtin_inff();
                 }
-                float next = top;
+                const float to_base2 = F32 ? __builtin_ldexpf(factor, -kshift) : c;
+                float next = -__builtin_inff();
 #pragma unroll
                 for (int j = 0; j < KB; j++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) next = fmaxf(next, sc[j][i]);
-                next = fmaxf(next, __shfl_xor(next, 32, 64));
+                next = fmaxf(next, __shfl_xor(next, 32, 64)) * to_base2;
                 if (__ballot(next > top)) {
-                    const float keep = exp2_hw((top - exp_base(next)) * c);
+                    next = fmaxf(next, top);
+                    const float keep = exp2_hw(top - exp_base(next));
                     l *= keep;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] *= keep;
                     top = next;
                 }
-                const float lift = exp_base(top) * c;
+                const float lift = exp_base(top) - PSHIFT;
 #pragma unroll
                 for (int j = 0; j < KB; j++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        sc[j][i] = exp2_hw(__builtin_fmaf(sc[j][i], c, -lift));
+                        sc[j][i] = exp2_hw(__builtin_fmaf(sc[j][i], to_base2, -lift));
                         l += sc[j][i];
                     }
 #pragma unroll
@@ -285,7 +350,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             E part[NP];
-                            split_parts(sc[j][8 * u + e], part);
+                            split_finite(sc[j][8 * u + e], part);
 #pragma unroll
                             for (int p = 0; p < NP; p++) pv[p][e] = part[p];
                         }
@@ -306,22 +371,23 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
                                 for (int p2 = NP - 1 - p; p2 >= 0; p2--) o[d] = mfma32(vt[p], pv[p2], o[d]);
                         }
                     }
-                if (s_odd[buf][1] == t + 1) {
+                if (s_odd[t & 1][1] == t + 1) {
                     // what was left out of the values, to the rows that see it
+                    const int h4 = kept_here(4 * h);
                     for (int key = base; key < base + BN; key++)
                         if (key < seen)
 #pragma unroll
                             for (int d = 0; d < DT; d++)
 #pragma unroll
                                 for (int i = 0; i < 16; i++) {
-                                    const float x = (float)vb[(int64_t)key * a.v_stride + 32 * d + 8 * (i / 4) + 4 * h + i % 4];
+                                    const float x = (float)vb[(int64_t)key * a.v_stride + 32 * d + 8 * (i / 4) + h4 + i % 4];
                                     if (!__builtin_isfinite(x)) o[d][i] += x;
                                 }
                 }
             }
-            if (NB == 1) {
-                __syncthreads();
-            } else if (t + 1 < tiles) {
+            if (t + 1 < tiles) {
+                look_through(t + 1);
+                if (NB == 1) __syncthreads();
                 store_tile(t + 1);
                 if (t + 2 < tiles) load_tile(t + 2);
             }
@@ -337,7 +403,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
                     typedef A Out __attribute__((ext_vector_type(4)));
                     Out x;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = (A)(l == 0.f ? 0.f : F32 ? o[d][i + e] / l : o[d][i + e] * inv);
+                    for (int e = 0; e < 4; e++) x[e] = (A)(l == 0.f ? 0.f : F32 ? __builtin_ldexpf(o[d][i + e] / l, -vshift) : o[d][i + e] * inv);
                     *(Out*)(out + 32 * d + 2 * i) = x;
                 }
         }

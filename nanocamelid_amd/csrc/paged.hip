@@ -588,6 +588,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                     __builtin_amdgcn_sched_barrier(0);
                     // the values left out go to the rows that see their key
                     if (__ballot(odd)) {
+                        const int g4 = kept_here(4 * g);
                         for (int key = 0; key < KW; key++) {
                             const int64_t at = s_off[buf][w][key];
                             if (at < 0) continue;
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                             for (int e = 0; e < ND; e++)
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {
-                                    const int d = F32 ? 64 * (e / 4) + 16 * g + 4 * i + e % 4 : ND * (4 * g + i) + e;
+                                    const int d = F32 ? 64 * (e / 4) + 4 * g4 + 4 * i + e % 4 : ND * (g4 + i) + e;
                                     const float v = (float)vb[at + d];
                                     if (!__builtin_isfinite(v))
 #pragma unroll
