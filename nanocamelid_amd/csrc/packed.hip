@@ -17,6 +17,7 @@ struct PackedParams {
     void* out;
     const int32_t *seq_start, *kv_start;
     int32_t seqs, rows, kv_rows, heads, kv_heads;
+    int32_t together;  // heads of a workgroup: 4, 2 or 1, as many as divide a group
     float scale;
 };
 
@@ -27,7 +28,7 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-constexpr int kPackedRows = 128;  // query rows of a workgroup, 32 a wave
+constexpr int kPackedRows = 32;  // query rows of a wave
 
 // The power of two that takes the float of these bits to [2^9, 2^10): small parts of such values are normal f16
 // numbers, sums of their products far from infinite.
@@ -45,8 +46,9 @@ __device__ __forceinline__ V4 read_columns(const void* p) {
     return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q));
 }
 
-// Attention of 128 query rows of one head over their sequence's keys, a tile of keys at a time with a running
-// maximum and sum.
+// Attention of 32 query rows of four heads that share a kv head (or 64 of two, 128 of one) over their sequence's
+// keys, a tile of keys at a time with a running maximum and sum.  Four heads together end their keys at one place,
+// which wastes less of the last tiles than four blocks of rows.
 //
 // Bound by the matrix products (4 head_dim operations a row and key) and, close behind, by the vector work of
 // the softmax.  Everything is transposed: scores^T = K q^T leaves a lane 16 scores of its own row for every 32
@@ -62,7 +64,7 @@ __device__ __forceinline__ V4 read_columns(const void* p) {
 //   factor and the answer give back.  The f32 products of the matrix cores run at a sixteenth of the f16 rate,
 //   these at a third.
 template <typename A, int HD>
-__global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a, int64_t units) {
+__global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packed_attention_kernel(PackedParams a, int64_t units) {
     constexpr bool F32 = sizeof(A) == 4;
     using E = std::conditional_t<F32, _Float16, A>;
     using V8 = typename Vec8<E>::type;
@@ -85,48 +87,41 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
 
     for (int64_t b = blockIdx.x; b < units; b += gridDim.x) {
         // the kv heads first, so that one head's workgroups share an XCD's L2
-        const int kvh = (int)(b % a.kv_heads), head = kvh * G + (int)(b / a.kv_heads % G);
-        int64_t tile = b / a.heads;
+        const int kvh = (int)(b % a.kv_heads), groups = G / a.together;
+        const int head = kvh * G + (int)(b / a.kv_heads % groups) * a.together + w % a.together;
+        const int high = 4 / a.together * kPackedRows;  // rows of the workgroup
+        int64_t tile = b / a.kv_heads / groups;
         // its sequence: tiles of 64 sequences at a time; a sequence's last rows, which see the most, first
         int s = -1, q0 = 0, begin = 0, n = 0;
         for (int s0 = 0; s0 < a.seqs; s0 += 64) {
             int mb = 0, mn = 0;
             if (s0 + lane < a.seqs) seq_rows(a.seq_start, s0 + lane, a.rows, mb, mn);
-            const int mine = (mn + kPackedRows - 1) / kPackedRows;
-            int upto = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const int x = __shfl_up(upto, d, 64);
-                if (lane >= d) upto += x;
-            }
+            const int upto = wave_prefix_sum((mn + high - 1) / high);
             const uint64_t past = __ballot(upto > tile);
             if (past) {
                 const int at = __builtin_ctzll(past);
                 s = s0 + at;
-                begin = __shfl(mb, at, 64);
-                n = __shfl(mn, at, 64);
-                q0 = (int)(__shfl(upto, at, 64) - 1 - tile) * kPackedRows;
+                begin = __builtin_amdgcn_readlane(mb, at);
+                n = __builtin_amdgcn_readlane(mn, at);
+                q0 = (__builtin_amdgcn_readlane(upto, at) - 1 - (int)tile) * high;
                 break;
             }
-            tile -= __shfl(upto, 63, 64);
+            tile -= __builtin_amdgcn_readlane(upto, 63);
         }
         if (s < 0) return;  // past the last tile, and so is every later one
         s = __builtin_amdgcn_readfirstlane(s);
         q0 = __builtin_amdgcn_readfirstlane(q0);
-        begin = __builtin_amdgcn_readfirstlane(begin);
-        n = __builtin_amdgcn_readfirstlane(n);
         int kbegin, m;
         seq_rows(a.kv_start, s, a.kv_rows, kbegin, m);
 
         // rows past the sequence's end take the last one's place and are not written
-        const int row = q0 + 32 * w + r < n ? q0 + 32 * w + r : n - 1;
+        const int first = q0 + w / a.together * kPackedRows;  // of the wave
+        const int row = first + r < n ? first + r : n - 1;
         const int before = m - n;  // may be negative
         const int seen = before + row + 1;
-        const int wave_last = q0 + 32 * w + 31 < n ? q0 + 32 * w + 31 : n - 1;
-        const int wave_most = before + wave_last + 1;                           // keys that some row of the wave sees
-        const int wave_least = before + (q0 + 32 * w < n ? q0 + 32 * w : n - 1) + 1;  // that every row sees
-        const int last = q0 + kPackedRows - 1 < n ? q0 + kPackedRows - 1 : n - 1;
-        const int most = before + last + 1;
+        const int wave_most = before + (first + 31 < n ? first + 31 : n - 1) + 1;  // keys that some row of the wave sees
+        const int wave_least = before + (first < n ? first : n - 1) + 1;           // that every row sees
+        const int most = before + (q0 + high - 1 < n ? q0 + high - 1 : n - 1) + 1;
         const int tiles = most > 0 ? (most + BN - 1) / BN : 0;
         const A* q = (const A*)a.q + (int64_t)(begin + row) * a.q_stride + head * HD;
         const A* kb = (const A*)a.k + (int64_t)kbegin * a.k_stride + kvh * HD;
@@ -279,6 +274,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
             const int base = t * BN;
             if (base < wave_most) {
                 f32x16 sc[KB] = {};
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int d = 0; d < KK; d++)
 #pragma unroll
@@ -292,6 +288,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
 #pragma unroll
                             for (int p2 = NP - 1 - p; p2 >= 0; p2--) sc[j] = mfma32(kv[p], qv[p2][d], sc[j]);
                     }
+                __builtin_amdgcn_s_setprio(0);
                 if (F32 && s_odd[t & 1][0] == t + 1) {
                     // keys that are not finite: parts of zero would make NaN of them, so their scores come from the
                     // rows themselves
@@ -313,11 +310,12 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
                         }
                 }
                 if (base + BN > wave_least) {
+                    const int own = kept_here(seen - base - 4 * h);  // a branch, not selects in every tile
 #pragma unroll
                     for (int j = 0; j < KB; j++)
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                            if (base + 32 * j + 8 * (i / 4) + 4 * h + i % 4 >= seen) sc[j][i] = -__builtin_inff();
+                            if (32 * j + 8 * (i / 4) + i % 4 >= own) sc[j][i] = -__builtin_inff();
                 }
                 const float to_base2 = F32 ? __builtin_ldexpf(factor, -kshift) : c;
                 float next = -__builtin_inff();
@@ -347,6 +345,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         V8 pv[NP];
+                        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             E part[NP];
@@ -371,6 +370,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
                                 for (int p2 = NP - 1 - p; p2 >= 0; p2--) o[d] = mfma32(vt[p], pv[p2], o[d]);
                         }
                     }
+                __builtin_amdgcn_s_setprio(0);
                 if (s_odd[t & 1][1] == t + 1) {
                     // what was left out of the values, to the rows that see it
                     const int h4 = kept_here(4 * h);
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedParams a
             }
         }
         l += __shfl_xor(l, 32, 64);
-        if (q0 + 32 * w + r < n) {
+        if (first + r < n) {
             const float inv = 1.f / l;
             A* out = (A*)a.out + ((int64_t)(begin + row) * a.heads + head) * HD + 4 * h;
 #pragma unroll
@@ -440,12 +440,14 @@ extern "C" int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t 
     if ((uintptr_t)out % 16 || (uintptr_t)seq_start % 4 || (uintptr_t)kv_start % 4)
         return fail(NC_EINVAL, "nc_packed_attention: misaligned output or starts");
     PackedParams a = {q, k, v, q_stride, k_stride, v_stride, out, seq_start, kv_start ? kv_start : seq_start, seqs,
-                      (int32_t)rows, (int32_t)kv_rows, heads, kv_heads, scale};
+                      (int32_t)rows, (int32_t)kv_rows, heads, kv_heads, 1, scale};
     DeviceGuard guard(ctx->device);
     if (guard.rc) return guard.rc;
     hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
+    const int group = heads / kv_heads;
+    a.together = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     // at most a tile more than its rows fill for every sequence; those past the last tile end at once
-    const int64_t units = (rows / kPackedRows + seqs) * heads;
+    const int64_t units = (rows / (4 / a.together * kPackedRows) + seqs) * (heads / a.together);
     const unsigned grid = (unsigned)std::min<int64_t>(units, 1 << 23);
     auto launch = [&]<typename A>() {
         if (head_dim == 64)
