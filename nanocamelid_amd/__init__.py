@@ -226,12 +226,13 @@ _ELEMENT_TYPES = {}
 
 
 def _element_type(who, t):
-    if not _ELEMENT_TYPES:
-        import torch
-        _ELEMENT_TYPES.update({torch.float32: NC_TYPE_F32, torch.float16: NC_TYPE_F16, torch.bfloat16: NC_TYPE_BF16})
     code = _ELEMENT_TYPES.get(t.dtype)
     if code is None:
-        raise NcError(NC_EINVAL, f"{who}: type must be float32, float16 or bfloat16")
+        import torch
+        _ELEMENT_TYPES.update({torch.float32: NC_TYPE_F32, torch.float16: NC_TYPE_F16, torch.bfloat16: NC_TYPE_BF16})
+        code = _ELEMENT_TYPES.get(t.dtype)
+        if code is None:
+            _refuse(who, "type must be float32, float16 or bfloat16")
     return code
 
 
@@ -240,38 +241,40 @@ def _refuse(who, why):
 
 
 def _int32(who, name, t, dims, device):
-    if t.dim() != dims or t.device != device or not t.is_contiguous() and (dims == 1 or t.stride(1) != 1):
-        _refuse(who, f"{name} must be a {dims}-dimensional tensor of contiguous rows on the cache's device")
-    if str(t.dtype) != "torch.int32":
+    import torch
+    if t.dim() != dims or t.device != device or dims == 1 and not t.is_contiguous() or dims == 2 and t.shape[1] > 1 and t.stride(1) != 1:
+        _refuse(who, f"{name} must be a {dims}-dimensional tensor of contiguous rows on the others' device")
+    if t.dtype != torch.int32:
         _refuse(who, f"{name} must be int32")
     return t.data_ptr()
 
 
-def _rows(who, name, t, heads, head_dim, like, rows=None):
-    """Row stride of packed rows [rows][heads][head_dim] whose heads lie end to end."""
-    if t.dtype != like.dtype or t.device != like.device:
-        _refuse(who, f"{name} must have the type and device of the other rows")
+def _rows(who, name, t, heads, head_dim, dtype, device, rows):
+    """Row stride of packed rows [rows][heads][head_dim] whose heads lie end to end.  device: a CUDA device's
+    index (get_device costs a third of a torch.device comparison); heads, rows: -1 for any."""
+    if t.dtype is not dtype or t.get_device() != device:
+        _refuse(who, f"{name} must have the rows' type and be on the context's device")
     shape = t.shape
-    if len(shape) != 3 or shape[2] != head_dim or heads is not None and shape[1] != heads or rows is not None and shape[0] != rows:
+    if len(shape) != 3 or shape[2] != head_dim or heads != shape[1] and heads >= 0 or rows != shape[0] and rows >= 0:
         _refuse(who, f"{name} has shape {tuple(shape)}")
     row, head, one = t.stride()
-    if (one != 1 and head_dim > 1) or (head != head_dim and shape[1] > 1):
+    if one != 1 or head != head_dim and shape[1] > 1:
         _refuse(who, f"the heads of a row of {name} must lie end to end")
     return row if shape[0] > 1 else shape[1] * head_dim
 
 
 def _output(who, name, out, like):
-    import torch
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+        return like.new_empty(like.shape)
+    if out.shape != like.shape or out.dtype is not like.dtype or out.device != like.device or not out.is_contiguous():
         _refuse(who, f"{name} must be contiguous, with the shape, type and device of its rows")
     return out
 
 
-def _on(who, ctx, t):
-    if t.device.type != "cuda" or t.device.index != ctx.device:
-        _refuse(who, "tensors must be on the context's device")
+def _same_device(who, ctx, *holders):
+    for x in holders:
+        if x.index != ctx.device:
+            _refuse(who, "the cache and the sequences must be on the context's device")
 
 
 class PagedKV:
@@ -294,7 +297,7 @@ class PagedKV:
         self.view = PagedKVView(k_pages.data_ptr(), v_pages.data_ptr(), pages, a, b, c, _element_type(who, k_pages), size,
                                 heads, hd)
         self.ref = C.byref(self.view)
-        self.kv_heads, self.head_dim, self.device, self.dtype = heads, hd, k_pages.device, k_pages.dtype
+        self.kv_heads, self.head_dim, self.index = heads, hd, k_pages.get_device()  # -1: not on a GPU
 
 
 class PagedBatch:
@@ -315,7 +318,7 @@ class PagedBatch:
                                    0 if row_start is None else _int32(who, "row_start", row_start, 1, device),
                                    table.stride(0) if seqs > 1 else pages, pages, seqs, max_len, 0)
         self.ref = C.byref(self.view)
-        self.table, self.lens, self.row_start, self.device = table, lens, row_start, device
+        self.table, self.lens, self.row_start, self.index = table, lens, row_start, table.get_device()
 
 
 def paged_kv_append(ctx: Context, cache: PagedKV, batch: PagedBatch, k, v, rope=None, q=None, want_k: bool = False,
@@ -325,31 +328,29 @@ def paged_kv_append(ctx: Context, cache: PagedKV, batch: PagedBatch, k, v, rope=
     rotates q [rows][heads][head_dim] alongside.  Rows may be views of a fused buffer: the heads of a row
     lie end to end, rows are 16-byte aligned.  Returns (rotated q or None, rotated k or None); k comes back
     where want_k or k_out asks for it.  q_out and k_out may be q and k themselves if those are contiguous."""
-    import torch
     who = "paged_kv_append"
-    _on(who, ctx, k)
-    if cache.device != k.device or batch.device != k.device:
-        _refuse(who, "the cache, the sequences and the rows must be on one device")
+    _same_device(who, ctx, cache, batch)
     code = _element_type(who, k)
-    hd, rows = cache.head_dim, k.shape[0]
-    ks = _rows(who, "k", k, cache.kv_heads, hd, k)
-    vs = _rows(who, "v", v, cache.kv_heads, hd, k, rows)
-    qs, heads, qp, qo = 0, 0, None, None
+    hd, dtype, device, rows = cache.head_dim, k.dtype, ctx.device, k.shape[0]
+    ks = _rows(who, "k", k, cache.kv_heads, hd, dtype, device, -1)
+    vs = _rows(who, "v", v, cache.kv_heads, hd, dtype, device, rows)
+    qs, heads, qp, qo, ko = 0, 0, None, None, None
     if q is not None:
-        qs = _rows(who, "q", q, None, hd, k, rows)
+        qs = _rows(who, "q", q, -1, hd, dtype, device, rows)
         heads, qp = q.shape[1], q.data_ptr()
         q_out = _output(who, "q_out", q_out, q)
         qo = q_out.data_ptr()
     if want_k or k_out is not None:
         k_out = _output(who, "k_out", k_out, k)
+        ko = k_out.data_ptr()
     rp, positions, dim = None, 0, 0
     if rope is not None:
-        if rope.dim() != 3 or rope.shape[2] != 2 or rope.dtype != torch.float32 or rope.device != k.device or not rope.is_contiguous():
-            _refuse(who, "rope must be a contiguous float32 [positions][rope_dim / 2][2] tensor on the rows' device")
-        rp, positions, dim = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
-    check(lib().nc_paged_kv_append(ctx.h, cache.ref, batch.ref, code, rows, k.data_ptr(), ks, v.data_ptr(), vs,
-                                   None if k_out is None else k_out.data_ptr(), qp, qs, heads, qo, rp, positions, dim,
-                                   _stream_of(k)))
+        shape = rope.shape
+        if len(shape) != 3 or shape[2] != 2 or rope.get_device() != device or not rope.is_contiguous() or str(rope.dtype) != "torch.float32":
+            _refuse(who, "rope must be a contiguous float32 [positions][rope_dim / 2][2] tensor on the context's device")
+        rp, positions, dim = rope.data_ptr(), shape[0], 2 * shape[1]
+    check(lib().nc_paged_kv_append(ctx.h, cache.ref, batch.ref, code, rows, k.data_ptr(), ks, v.data_ptr(), vs, ko, qp, qs, heads,
+                                   qo, rp, positions, dim, _stream_of(k)))
     return (q_out if q is not None else None), k_out
 
 
@@ -361,21 +362,22 @@ def paged_attention(ctx: Context, cache: PagedKV, batch: PagedBatch, q, scale: f
     graphs, share none."""
     import torch
     who = "paged_attention"
-    _on(who, ctx, q)
-    if cache.device != q.device or batch.device != q.device:
-        _refuse(who, "the cache, the sequences and the rows must be on one device")
+    _same_device(who, ctx, cache, batch)
     code = _element_type(who, q)
     hd = cache.head_dim
-    qs = _rows(who, "q", q, None, hd, q)
+    qs = _rows(who, "q", q, -1, hd, q.dtype, ctx.device, -1)
     rows, heads = q.shape[0], q.shape[1]
     out = _output(who, "out", out, q)
-    need = lib().nc_paged_attention_work_bytes(cache.ref, batch.ref, rows, heads)
-    if need < 0:
+    L = lib()
+    need = L.nc_paged_attention_work_bytes(cache.ref, batch.ref, rows, heads)
+    work = None
+    if need > 0:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif need < 0:
         check(int(need))
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(lib().nc_paged_attention(ctx.h, cache.ref, batch.ref, code, rows, q.data_ptr(), qs, heads,
-                                   hd ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                                   None if work is None else work.data_ptr(), need, _stream_of(q)))
+    check(L.nc_paged_attention(ctx.h, cache.ref, batch.ref, code, rows, q.data_ptr(), qs, heads,
+                               hd ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                               None if work is None else work.data_ptr(), need, _stream_of(q)))
     return out
 
 
@@ -386,14 +388,15 @@ def packed_attention(ctx: Context, q, k, v, seq_start, kv_start=None, scale: flo
     a sequence sees all of its keys, the one before all but the last, and so on.  Rows may be views of a fused
     buffer.  Returns [rows][heads][head_dim]; rows outside every sequence are left as they were in out."""
     who = "packed_attention"
-    _on(who, ctx, q)
     code = _element_type(who, q)
     if q.dim() != 3 or k.dim() != 3 or seq_start.dim() != 1 or seq_start.shape[0] < 1:
         _refuse(who, "rows are [rows][heads][head_dim], starts [seqs + 1]")
-    hd, kv = q.shape[2], k.shape[1]
-    qs = _rows(who, "q", q, None, hd, q)
-    ks = _rows(who, "k", k, kv, hd, q)
-    vs = _rows(who, "v", v, kv, hd, q, k.shape[0])
+    rows, heads, hd = q.shape
+    kv_rows, kv, _ = k.shape
+    dtype, device = q.dtype, ctx.device
+    qs = _rows(who, "q", q, heads, hd, dtype, device, rows)
+    ks = _rows(who, "k", k, kv, hd, dtype, device, kv_rows)
+    vs = _rows(who, "v", v, kv, hd, dtype, device, kv_rows)
     starts = _int32(who, "seq_start", seq_start, 1, q.device)
     kstarts = None
     if kv_start is not None:
@@ -401,9 +404,9 @@ def packed_attention(ctx: Context, q, k, v, seq_start, kv_start=None, scale: flo
             _refuse(who, "kv_start must have seq_start's shape")
         kstarts = _int32(who, "kv_start", kv_start, 1, q.device)
     out = _output(who, "out", out, q)
-    check(lib().nc_packed_attention(ctx.h, code, q.shape[0], k.shape[0], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-                                    q.shape[1], kv, hd, starts, kstarts, seq_start.shape[0] - 1,
-                                    hd ** -0.5 if scale is None else float(scale), out.data_ptr(), _stream_of(q)))
+    check(lib().nc_packed_attention(ctx.h, code, rows, kv_rows, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, heads, kv, hd,
+                                    starts, kstarts, seq_start.shape[0] - 1, hd ** -0.5 if scale is None else float(scale),
+                                    out.data_ptr(), _stream_of(q)))
     return out
 
 
