@@ -7,6 +7,7 @@
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
 
 #ifdef __HIP__
 #define NC_PAGED_HD __host__ __device__ __forceinline__
@@ -183,6 +184,40 @@ struct Vec8<__bf16> {
 __device__ __forceinline__ int kept_here(int x) {
     asm volatile("" : "+v"(x));
     return x;
+}
+
+// A lane's value and that of the lane 16 or 32 from it, in some order: the swap exchanges every other row of 16
+// lanes, or half of 32, of two registers, here of one and the same value.
+template <int APART>
+__device__ __forceinline__ f32x2 with_lane_across(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = APART == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return f32x2{__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+template <int APART>
+__device__ __forceinline__ float max_across(float x) {
+    const f32x2 v = with_lane_across<APART>(x);
+    return fmaxf(v[0], v[1]);
+}
+template <int APART>
+__device__ __forceinline__ float sum_across(float x) {
+    const f32x2 v = with_lane_across<APART>(x);
+    return v[0] + v[1];
+}
+
+// The wave's largest of v.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    auto up = [&](auto dpp) {
+        const uint32_t x = __builtin_amdgcn_update_dpp(0, v, decltype(dpp)::value, 0xf, 0xf, false);
+        v = x > v ? x : v;
+    };
+    up(std::integral_constant<int, 0x111>());  // row_shr:1, 2, 4, 8, then row_bcast:15 and 31 (lanes without a
+    up(std::integral_constant<int, 0x112>());  // source see 0)
+    up(std::integral_constant<int, 0x114>());
+    up(std::integral_constant<int, 0x118>());
+    up(std::integral_constant<int, 0x142>());
+    up(std::integral_constant<int, 0x143>());
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 // The sum of v over the lanes up to the own one: within rows of 16 lanes, then the rows' last ones onto the next.

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[d][e]));
             }
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            top = max_across<32>(top);
             const int shift = shift_of(__float_as_uint(top));
             factor = __builtin_ldexpf(c, -shift);
 #pragma unroll
@@ -205,9 +205,8 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
                 for (int i = 0; i < NL; i++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) kt = fmaxf(kt, __builtin_fabsf(kx[i][e])), vt = fmaxf(vt, __builtin_fabsf(vx[i][e]));
-#pragma unroll
-                for (int d = 1; d < 64; d *= 2) kt = fmaxf(kt, __shfl_xor(kt, d, 64)), vt = fmaxf(vt, __shfl_xor(vt, d, 64));
-                if (lane == 0) s_top[w][0] = __float_as_uint(kt), s_top[w][1] = __float_as_uint(vt);
+                const uint32_t kw = wave_max(__float_as_uint(kt)), vw = wave_max(__float_as_uint(vt));
+                if (lane == 0) s_top[w][0] = kw, s_top[w][1] = vw;
             }
         };
         auto store_tile = [&](int t) {
@@ -323,7 +322,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
                 for (int j = 0; j < KB; j++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) next = fmaxf(next, sc[j][i]);
-                next = fmaxf(next, __shfl_xor(next, 32, 64)) * to_base2;
+                next = max_across<32>(next) * to_base2;
                 if (__ballot(next > top)) {
                     next = fmaxf(next, top);
                     const float keep = exp2_hw(top - exp_base(next));
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
                 if (t + 2 < tiles) load_tile(t + 2);
             }
         }
-        l += __shfl_xor(l, 32, 64);
+        l = sum_across<32>(l);
         if (first + r < n) {
             const float inv = 1.f / l;
             A* out = (A*)a.out + ((int64_t)(begin + row) * a.heads + head) * HD + 4 * h;

@@ -259,23 +259,18 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
             for (int s0 = 0; s0 < a.seqs.seqs; s0 += 64) {
                 int mb = 0, mn = 0;
                 if (s0 + lane < a.seqs.seqs) seq_rows(row_start, s0 + lane, a.seqs.rows, mb, mn);
-                int upto = (mn * G + 16 * RT - 1) / (16 * RT);
-#pragma unroll
-                for (int d = 1; d < 64; d *= 2) {
-                    const int x = __shfl_up(upto, d, 64);
-                    if (lane >= d) upto += x;
-                }
+                const int upto = wave_prefix_sum((mn * G + 16 * RT - 1) / (16 * RT));
                 const uint64_t past = __ballot(upto > u);
                 if (past) {
                     const int at = __builtin_ctzll(past);
                     s = s0 + at;
-                    begin = __builtin_amdgcn_readfirstlane(__shfl(mb, at, 64));
-                    n = __builtin_amdgcn_readfirstlane(__shfl(mn, at, 64));
+                    begin = __builtin_amdgcn_readlane(mb, at);
+                    n = __builtin_amdgcn_readlane(mn, at);
                     // counted from the sequence's last group
-                    r0 = __builtin_amdgcn_readfirstlane((int)(__shfl(upto, at, 64) - 1 - u)) * (16 * RT);
+                    r0 = (__builtin_amdgcn_readlane(upto, at) - 1 - (int)u) * (16 * RT);
                     break;
                 }
-                u -= __shfl(upto, 63, 64);
+                u -= __builtin_amdgcn_readlane(upto, 63);
             }
             if (s < 0) return;  // past the last unit, and so is every later one
             s = __builtin_amdgcn_readfirstlane(s);
@@ -382,8 +377,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                     }
                     int shift = 0;
                     if (QSCALE) {  // the row's largest value to [2^9, 2^10)
-                        top = fmaxf(top, __shfl_xor(top, 16, 64));
-                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        top = max_across<32>(max_across<16>(top));
                         const int ex = (int)(__float_as_uint(top) >> 23);
                         shift = ex == 0 || ex == 255 ? 0 : 136 - ex;
                         factor = __builtin_ldexpf(factor, -shift);
@@ -495,8 +489,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                         for (int j = 0; j < KT; j++)
 #pragma unroll
                             for (int i = 0; i < 4; i++) top = fmaxf(top, sc[t][j][i]);
-                        top = fmaxf(top, __shfl_xor(top, 16, 64));
-                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        top = max_across<32>(max_across<16>(top));
                         const float lift = exp_base(top) - PSHIFT;
                         float total = 0.f;
 #pragma unroll
@@ -507,8 +500,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(P
                                 sc[t][j][i] = e;
                                 total += e;
                             }
-                        total += __shfl_xor(total, 16, 64);
-                        total += __shfl_xor(total, 32, 64);
+                        total = sum_across<32>(sum_across<16>(total));
                         m[t] = top;
                         l[t] = total;
                     }
