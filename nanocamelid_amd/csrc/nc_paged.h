@@ -157,7 +157,7 @@ __device__ __forceinline__ void split_finite(float x, T (&part)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
         part[i] = (T)x;
-        x -= (float)part[i];
+        if (i + 1 < N) x = __builtin_fmaf((float)part[i], -1.f, x);  // exact; one instruction takes the 16-bit operand
     }
 }
 

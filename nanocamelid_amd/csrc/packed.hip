@@ -63,8 +63,8 @@ __device__ __forceinline__ V4 read_columns(const void* p) {
 //   of queries by its largest, keys and values by the largest so far, which is a power of two that the scores'
 //   factor and the answer give back.  The f32 products of the matrix cores run at a sixteenth of the f16 rate,
 //   these at a third.
-template <typename A, int HD>
-__global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packed_attention_kernel(PackedParams a, int64_t units) {
+template <typename A, int HD, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ? 3 : 2) void packed_attention_kernel(PackedParams a, int64_t units) {
     constexpr bool F32 = sizeof(A) == 4;
     using E = std::conditional_t<F32, _Float16, A>;
     using V8 = typename Vec8<E>::type;
@@ -74,11 +74,11 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
     constexpr int BN = F32 ? 32 : 64;      // keys of a tile
     constexpr int NB = F32 ? 1 : 2;        // LDS buffers
     constexpr int PC = HD / 8;             // 16-byte pieces of an LDS row
-    constexpr int NL = BN * PC / 256;      // pieces of a tile that a thread moves
+    constexpr int NL = BN * PC / (64 * NW);  // pieces of a tile that a thread moves
     constexpr int KB = BN / 32, DT = HD / 32, KK = HD / 16;
     __shared__ __attribute__((aligned(16))) E s_k[NB][NP][BN][HD], s_v[NB][NP][BN][HD];
     __shared__ int s_odd[2][2];           // by the tile's parity: the tile (from 1) whose keys, values held an infinity or NaN
-    __shared__ uint32_t s_top[4][2];      // f32: the largest of the next tile's keys, values that each wave moves
+    __shared__ uint32_t s_top[NW][2];      // f32: the largest of the next tile's keys, values that each wave moves
 
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, h = lane >> 5;
     const int G = a.heads / a.kv_heads;
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
         // the kv heads first, so that one head's workgroups share an XCD's L2
         const int kvh = (int)(b % a.kv_heads), groups = G / a.together;
         const int head = kvh * G + (int)(b / a.kv_heads % groups) * a.together + w % a.together;
-        const int high = 4 / a.together * kPackedRows;  // rows of the workgroup
+        const int high = NW / a.together * kPackedRows;  // rows of the workgroup
         int64_t tile = b / a.kv_heads / groups;
         // its sequence: tiles of 64 sequences at a time; a sequence's last rows, which see the most, first
         int s = -1, q0 = 0, begin = 0, n = 0;
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
         auto load_tile = [&](int t) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int id = tid + 256 * i, key = t * BN + id / PC;
+                const int id = tid + 64 * NW * i, key = t * BN + id / PC;
                 const int64_t at = key < most ? key : most - 1;
                 kx[i] = *(const Raw*)(kb + at * a.k_stride + id % PC * 8);
                 vx[i] = *(const Raw*)(vb + at * a.v_stride + id % PC * 8);
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
             if constexpr (F32) {
                 uint32_t kt = 0, vt = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < NW; i++) {
                     kt = kt > s_top[i][0] ? kt : s_top[i][0];
                     vt = vt > s_top[i][1] ? vt : s_top[i][1];
                 }
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
             }
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int id = tid + 256 * i, key = id / PC, piece = id % PC;
+                const int id = tid + 64 * NW * i, key = id / PC, piece = id % PC;
                 const int pk = (piece ^ (key & (PC - 1))) * 8, pv = (piece ^ (2 * key & (PC - 1))) * 8;
                 if constexpr (F32) {
                     V8 kp[NP], vp[NP];
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256, HD == 64 && sizeof(A) == 2 ? 3 : 2) void packe
                     typedef A Out __attribute__((ext_vector_type(4)));
                     Out x;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = (A)(l == 0.f ? 0.f : F32 ? __builtin_ldexpf(o[d][i + e] / l, -vshift) : o[d][i + e] * inv);
+                    for (int e = 0; e < 4; e++) x[e] = (A)(l == 0.f ? 0.f : F32 ? __builtin_ldexpf(o[d][i + e] * inv, -vshift) : o[d][i + e] * inv);
                     *(Out*)(out + 32 * d + 2 * i) = x;
                 }
         }
@@ -446,17 +446,17 @@ extern "C" int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t 
     const int group = heads / kv_heads;
     a.together = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     // at most a tile more than its rows fill for every sequence; those past the last tile end at once
-    const int64_t units = (rows / (4 / a.together * kPackedRows) + seqs) * (heads / a.together);
-    const unsigned grid = (unsigned)std::min<int64_t>(units, 1 << 23);
-    auto launch = [&]<typename A>() {
-        if (head_dim == 64)
-            packed_attention_kernel<A, 64><<<grid, 256, 0, st>>>(a, units);
-        else
-            packed_attention_kernel<A, 128><<<grid, 256, 0, st>>>(a, units);
+    auto launch = [&]<typename A, int HD, int NW>() {
+        const int64_t units = (rows / (NW / a.together * kPackedRows) + seqs) * (heads / a.together);
+        packed_attention_kernel<A, HD, NW><<<(unsigned)std::min<int64_t>(units, 1 << 22), 64 * NW, 0, st>>>(a, units);
         NC_HIP(hipGetLastError());
         return (int)NC_OK;
     };
-    if (type == NC_TYPE_F32) return launch.template operator()<float>();
-    if (type == NC_TYPE_F16) return launch.template operator()<_Float16>();
-    return launch.template operator()<__bf16>();
+    if (type == NC_TYPE_F16) return head_dim == 64 ? launch.template operator()<_Float16, 64, 4>() : launch.template operator()<_Float16, 128, 4>();
+    if (type == NC_TYPE_BF16) return head_dim == 64 ? launch.template operator()<__bf16, 64, 4>() : launch.template operator()<__bf16, 128, 4>();
+    if (head_dim == 64) return launch.template operator()<float, 64, 4>();
+    // Eight waves share the splitting of a tile, a third of a wave's vector work, as long as that does not take more
+    // than 64 rows of a sequence together (4096 rows, 32 heads over 8: 458 us with eight, 493 with four; six prompts
+    // of up to 1200 rows, 24 heads over 8: 216 and 207).
+    return a.together == 4 ? launch.template operator()<float, 128, 8>() : launch.template operator()<float, 128, 4>();
 }

@@ -43,7 +43,7 @@ def _check(out, q, k, v, rows, keys, scale):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=ids)
-@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 128), (3, 3, 64), (8, 1, 64), (5, 1, 128)])
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 128), (3, 3, 64), (8, 1, 64), (5, 1, 128), (8, 2, 128), (12, 1, 64)])
 def test_ragged_prompts(ctx, dtype, heads, kv, hd):
     rows = [1, 2, 31, 32, 33, 0, 63, 64, 65, 127, 128, 129, 16, 17, 200]
     q, k, v = _fused(sum(rows), heads, kv, hd, 1, dtype)
@@ -53,29 +53,31 @@ def test_ragged_prompts(ctx, dtype, heads, kv, hd):
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=ids)
 @pytest.mark.parametrize("n,hd", [(1, 128), (255, 64), (256, 128), (257, 128), (513, 64), (770, 128)])
-def test_one_prompt(ctx, dtype, n, hd):
-    q, k, v = _fused(n, 2, 1, hd, 2 + n, dtype)
+@pytest.mark.parametrize("heads", [2, 4])
+def test_one_prompt(ctx, dtype, n, hd, heads):
+    q, k, v = _fused(n, heads, 1, hd, 2 + n, dtype)
     out = nc.packed_attention(ctx, q, k, v, ints([0, n]))
     _check(out, q, k, v, [n], [n], hd**-0.5)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
-@pytest.mark.parametrize("hd", [64, 128])
-def test_continued_prompts_and_rows_that_see_nothing(ctx, dtype, hd):
+@pytest.mark.parametrize("hd,heads", [(64, 4), (128, 4), (128, 8)])
+def test_continued_prompts_and_rows_that_see_nothing(ctx, dtype, hd, heads):
     """More keys than rows (a prompt that goes on), fewer (the first rows see none), none at all."""
     rows, keys = [5, 130, 40, 10, 7, 64, 0], [300, 131, 33, 0, 7, 129, 20]
     a = starts(rows)
-    q = _randn((sum(rows), 4, hd), 11, 1.3, dtype)
+    q = _randn((sum(rows), heads, hd), 11, 1.3, dtype)
     k, v = _randn((sum(keys), 2, hd), 12, 1.0, dtype), _randn((sum(keys), 2, hd), 13, 1.0, dtype)
     out = nc.packed_attention(ctx, q, k, v, ints(a), ints(starts(keys)))
     _check(out, q, k, v, rows, keys, hd**-0.5)
     assert (out[a[2]:a[2] + 7] == 0).all() and (out[a[3]:a[4]] == 0).all()
 
 
+@pytest.mark.parametrize("heads", [4, 8])
 @pytest.mark.parametrize("dtype", [F32, F16], ids=ids)
-def test_neighbours_do_not_leak(ctx, dtype):
+def test_neighbours_do_not_leak(ctx, dtype, heads):
     """What other sequences and the rows between them hold, NaN and infinities too, reaches no row."""
-    q, k, v = (x.contiguous() for x in _fused(200, 4, 2, 128, 21, dtype))
+    q, k, v = (x.contiguous() for x in _fused(200, heads, 2, 128, 21, dtype))
     alone = nc.packed_attention(ctx, q[70:130].contiguous(), k[70:130].contiguous(), v[70:130].contiguous(), ints([0, 60]))
     for x in (k, v):
         x[:70], x[130:] = math.nan, math.inf
@@ -84,9 +86,10 @@ def test_neighbours_do_not_leak(ctx, dtype):
     assert torch.equal(out[70:130], alone) and (out[:70] == 3).all() and (out[130:] == 3).all()
 
 
-def test_causal_mask_hides_infinities(ctx):
+@pytest.mark.parametrize("dtype,heads,hd", [(F32, 2, 128), (F32, 4, 128), (F32, 4, 64), (F16, 2, 64), (BF16, 4, 128)], ids=ids)
+def test_causal_mask_hides_infinities(ctx, dtype, heads, hd):
     """A row sees nothing of the later rows, whatever they hold."""
-    q, k, v = (x.contiguous() for x in _fused(150, 2, 1, 128, 31, F32))
+    q, k, v = (x.contiguous() for x in _fused(150, heads, 1, hd, 31, dtype))
     want = nc.packed_attention(ctx, q, k, v, ints([0, 150]))
     k2, v2 = k.clone(), v.clone()
     k2[100:], v2[100:] = math.inf, math.nan
@@ -94,15 +97,33 @@ def test_causal_mask_hides_infinities(ctx):
     assert torch.equal(got[:100], want[:100]) and torch.isnan(got[100:]).all()
 
 
-def test_extreme_scores(ctx):
-    q, k, v = (x.contiguous() for x in _fused(140, 2, 1, 64, 41, F32))
+@pytest.mark.parametrize("heads,hd", [(2, 64), (4, 128)])
+def test_extreme_scores(ctx, heads, hd):
+    q, k, v = (x.contiguous() for x in _fused(140, heads, 1, hd, 41, F32))
     k[3] *= 50
     k[90] *= 70
     out = nc.packed_attention(ctx, q, k, v, ints([0, 140]))
-    _check(out, q, k, v, [140], [140], 0.125)
+    _check(out, q, k, v, [140], [140], hd**-0.5)
     q[:] = 1.0
     k[:] = -math.inf
     assert (nc.packed_attention(ctx, q, k, v, ints([0, 140])) == 0).all()
+
+
+@pytest.mark.parametrize("heads,hd", [(2, 64), (4, 128)])
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 3e4, 1e15])
+def test_f32_values_of_any_size(ctx, heads, hd, size):
+    """Sizes far from one, and sizes that grow and shrink along the sequence: relative accuracy holds."""
+    q, k, v = (x.contiguous() for x in _fused(200, heads, 1, hd, 45, F32))
+    k, v, q = k * size, v * size, q / size
+    _check(nc.packed_attention(ctx, q, k, v, ints([0, 200])), q, k, v, [200], [200], hd**-0.5)
+    # values by row: tiny ones first, large ones later, which rows before them must not feel
+    grow = (10.0 ** torch.linspace(-4, 4, 200)).cuda()[:, None, None]
+    v = v * grow
+    out = nc.packed_attention(ctx, q, k, v, ints([0, 200]))
+    rows = [40, 80, 120, 160, 200]
+    for n in rows:
+        want, tol = attend(q[n - 1:n], k[:n], v[:n], hd**-0.5)
+        close(out[n - 1:n], want, tol, n)
 
 
 def test_scale(ctx):
