@@ -220,6 +220,20 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+// The largest of v in each group of 8 or 16 lanes, in the group's last lane.
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    auto up = [&](auto dpp) {
+        const uint32_t x = __builtin_amdgcn_update_dpp(0, v, decltype(dpp)::value, 0xf, 0xf, false);
+        v = x > v ? x : v;
+    };
+    up(std::integral_constant<int, 0x111>());
+    up(std::integral_constant<int, 0x112>());
+    up(std::integral_constant<int, 0x114>());
+    if (LANES == 16) up(std::integral_constant<int, 0x118>());
+    return v;
+}
+
 // The sum of v over the lanes up to the own one: within rows of 16 lanes, then the rows' last ones onto the next.
 __device__ __forceinline__ int wave_prefix_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8

@@ -30,12 +30,13 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 
 constexpr int kPackedRows = 32;  // query rows of a wave
 
-// The power of two that takes the float of these bits to [2^9, 2^10): small parts of such values are normal f16
-// numbers, sums of their products far from infinite.
+// The power of two that takes the float of these bits to [2^14, 2^15): the two f16 parts of such a value hold 24
+// bits down to 2^-16 of it, and sums of their products are far from infinite.  0 for zero and what is not finite.
 __device__ __forceinline__ int shift_of(uint32_t bits) {
     const int ex = (int)(bits >> 23) & 255;
-    return ex == 0 || ex == 255 ? 0 : 136 - ex;
+    return ex == 0 || ex == 255 ? 0 : 141 - ex;
 }
+constexpr uint32_t kInfBits = 0x7f800000u;
 
 // Four keys' values of one dimension: the 16 lanes of a group read four rows of 16 dimensions, eight bytes each,
 // and get a column back.
@@ -59,10 +60,11 @@ __device__ __forceinline__ V4 read_columns(const void* p) {
 //   16 bits: values are read as columns by the transposing LDS read, weights are rounded to the operands' type
 //   (as much as the answer's own rounding).
 //   f32: keys, values, queries and weights as two f16 parts (nc_paged.h), of whose products the smallest is left
-//   out, below 2^-24 of |q||k|.  Parts keep their bits for values down to 2^-16 of what they are scaled by: a row
-//   of queries by its largest, keys and values by the largest so far, which is a power of two that the scores'
-//   factor and the answer give back.  The f32 products of the matrix cores run at a sixteenth of the f16 rate,
-//   these at a third.
+//   out, below 2^-24 of |q||k|.  Parts hold a value's 24 bits down to 2^-16 of what it is scaled by: a row of
+//   queries by its largest, a tile's keys by theirs, values by the largest so far, in powers of two that the
+//   scores' factor and the answer give back.  The f32 products of the matrix cores run at a sixteenth of the f16
+//   rate, these at a third.  Where keys or values of a tile differ in size by more (a huge one that only later rows
+//   see, say), or one is not finite, the tile takes the f32 products.
 template <typename A, int HD, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ? 3 : 2) void packed_attention_kernel(PackedParams a, int64_t units) {
     constexpr bool F32 = sizeof(A) == 4;
@@ -77,8 +79,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
     constexpr int NL = BN * PC / (64 * NW);  // pieces of a tile that a thread moves
     constexpr int KB = BN / 32, DT = HD / 32, KK = HD / 16;
     __shared__ __attribute__((aligned(16))) E s_k[NB][NP][BN][HD], s_v[NB][NP][BN][HD];
-    __shared__ int s_odd[2][2];           // by the tile's parity: the tile (from 1) whose keys, values held an infinity or NaN
-    __shared__ uint32_t s_top[NW][2];      // f32: the largest of the next tile's keys, values that each wave moves
+    __shared__ int s_odd[2];  // by the tile's parity: the tile (from 1) of whose values some were left out
+    __shared__ __attribute__((aligned(16))) uint32_t s_size[NW][4];  // f32: of the next tile's keys and values that a wave moves
 
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, h = lane >> 5;
     const int G = a.heads / a.kv_heads;
@@ -172,61 +174,114 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
             }
         };
         f32x16 o[DT] = {};
-        // f32: what keys and values are scaled by, 2^shift of the largest so far; no tile has asked yet
-        int kshift = 1000, vshift = 1000;
-        // Values behind the last key or not finite are left out of the product (a zero weight times them would be no
-        // zero): f32 tiles are looked through before they are split, 16-bit ones where rows mask keys.  f32: then the
-        // wave's largest key and value.
-        auto look_through = [&](int t) {
-            const bool edge = (t + 1) * BN > before + q0 + 1;
-            if (!F32 && !edge) return;
-            float kodd = 0.f, vodd = 0.f;  // NaN if there is one
+        // f32: keys are scaled by 2^kshift, a tile's own, values by 2^vshift, that of the largest so far (1000: none but
+        // zeros yet).  A rough tile is one that f16 parts cannot hold together.
+        int kshift = 0, vshift = 1000;
+        bool rough = false;
+        // A zero weight times a value that is not finite is no zero: such values are left out of the product, f32 ones
+        // always, 16-bit ones where rows mask keys.
+        auto leave_out = [&](int t) {
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < NL; i++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if (F32) kodd = __builtin_fmaf((float)kx[i][e], 0.f, kodd);
-                    vodd = __builtin_fmaf((float)vx[i][e], 0.f, vodd);
-                }
-            if (__ballot(kodd != kodd || vodd != vodd)) {
-                if (kodd != kodd) s_odd[t & 1][0] = t + 1;
-                if (vodd != vodd) s_odd[t & 1][1] = t + 1;
-#pragma unroll
-                for (int i = 0; i < NL; i++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        if (F32 && !__builtin_isfinite((float)kx[i][e])) kx[i][e] = (A)0.f;
-                        if (!__builtin_isfinite((float)vx[i][e])) vx[i][e] = (A)0.f;
+                for (int e = 0; e < 8; e++)
+                    if (!__builtin_isfinite((float)vx[i][e])) {
+                        vx[i][e] = (A)0.f;
+                        any = true;
                     }
-            }
+            if (any) s_odd[t & 1] = t + 1;
+        };
+        auto look_through = [&](int t) {
             if constexpr (F32) {
-                float kt = 0.f, vt = 0.f;
+                // the largest of every key's and value's dimensions, as bits, which order as the sizes do, infinities
+                // and NaN last; of them the wave's largest, and its smallest but zero
+                uint32_t km[NL], vm[NL];
+                auto sizes = [&]() {
+#pragma unroll
+                    for (int i = 0; i < NL; i++) {
+                        km[i] = vm[i] = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const uint32_t x = __float_as_uint(kx[i][e]) & 0x7fffffffu, y = __float_as_uint(vx[i][e]) & 0x7fffffffu;
+                            km[i] = km[i] > x ? km[i] : x;
+                            vm[i] = vm[i] > y ? vm[i] : y;
+                        }
+                        km[i] = group_max<PC>(km[i]);
+                        vm[i] = group_max<PC>(vm[i]);
+                    }
+                };
+                sizes();
+                uint32_t big = 0;
+#pragma unroll
+                for (int i = 0; i < NL; i++) big = big > vm[i] ? big : vm[i];
+                if (__ballot(big >= kInfBits)) {
+                    leave_out(t);
+                    sizes();
+                }
+                uint32_t kt = 0, vt = 0, kl = ~0u, vl = ~0u;
+#pragma unroll
+                for (int i = 0; i < NL; i++) {
+                    kt = kt > km[i] ? kt : km[i];
+                    vt = vt > vm[i] ? vt : vm[i];
+                    if (lane % PC == PC - 1) {  // where the group's maximum is
+                        kl = km[i] != 0 && km[i] < kl ? km[i] : kl;
+                        vl = vm[i] != 0 && vm[i] < vl ? vm[i] : vl;
+                    }
+                }
+                kt = wave_max(kt);
+                vt = wave_max(vt);
+                kl = ~wave_max(~kl);
+                vl = ~wave_max(~vl);
+                if (lane == 0) *(u32x4*)s_size[w] = u32x4{kt, vt, kl, vl};
+            } else if ((t + 1) * BN > before + q0 + 1) {
+                float odd = 0.f;  // NaN if there is one
 #pragma unroll
                 for (int i = 0; i < NL; i++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) kt = fmaxf(kt, __builtin_fabsf(kx[i][e])), vt = fmaxf(vt, __builtin_fabsf(vx[i][e]));
-                const uint32_t kw = wave_max(__float_as_uint(kt)), vw = wave_max(__float_as_uint(vt));
-                if (lane == 0) s_top[w][0] = kw, s_top[w][1] = vw;
+                    for (int e = 0; e < 8; e++) odd = __builtin_fmaf((float)vx[i][e], 0.f, odd);
+                if (__ballot(odd != odd)) leave_out(t);
             }
         };
         auto store_tile = [&](int t) {
             const int buf = NB == 2 ? t & 1 : 0;
             if constexpr (F32) {
-                uint32_t kt = 0, vt = 0;
+                u32x4 size = *(const u32x4*)s_size[0];
 #pragma unroll
-                for (int i = 0; i < NW; i++) {
-                    kt = kt > s_top[i][0] ? kt : s_top[i][0];
-                    vt = vt > s_top[i][1] ? vt : s_top[i][1];
+                for (int i = 1; i < NW; i++) {
+                    const u32x4 x = *(const u32x4*)s_size[i];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        size[e] = x[e] > size[e] ? x[e] : size[e];
+                        size[2 + e] = x[2 + e] < size[2 + e] ? x[2 + e] : size[2 + e];
+                    }
                 }
-                const int ks = shift_of(kt), vs = shift_of(vt);
-                kshift = ks < kshift ? ks : kshift;
-                if (vs < vshift) {
-                    if (vshift != 1000)
+                // one key or value 2^16 times another, or a key that is not finite
+                rough = size[0] >= kInfBits || (size[0] != 0 && (size[0] >> 23) - (size[2] >> 23) > 16) ||
+                        (size[1] != 0 && (size[1] >> 23) - (size[3] >> 23) > 16);
+                kshift = shift_of(size[0]);
+                if (size[1] != 0) {
+                    const int vs = shift_of(size[1]);
+                    if (vs > vshift + 16) {
+                        rough = true;  // all far below what came before
+                    } else if (vs < vshift) {
+                        if (vshift != 1000)
 #pragma unroll
-                        for (int d = 0; d < DT; d++)
+                            for (int d = 0; d < DT; d++)
 #pragma unroll
-                            for (int i = 0; i < 16; i++) o[d][i] = __builtin_ldexpf(o[d][i], vs - vshift);
-                    vshift = vs;
+                                for (int i = 0; i < 16; i++) o[d][i] = __builtin_ldexpf(o[d][i], vs - vshift);
+                        vshift = vs;
+                    }
+                }
+                if (rough) {
+                    // the tile as it is, in the same place
+#pragma unroll
+                    for (int i = 0; i < NL; i++) {
+                        const int at = (tid + 64 * NW * i) * 8;
+                        *(Raw*)((float*)s_k + at) = kx[i];
+                        *(Raw*)((float*)s_v + at) = vx[i];
+                    }
+                    return;
                 }
             }
 #pragma unroll
@@ -258,7 +313,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
         };
 
         float top = -__builtin_inff(), l = 0.f;  // of the row; l of the lane's own keys
-        if (tid < 4) s_odd[tid / 2][tid % 2] = 0;
+        if (tid < 2) s_odd[tid] = 0;
         if (tiles > 0) load_tile(0);
         __syncthreads();
         if (tiles > 0) {
@@ -274,40 +329,26 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
             if (base < wave_most) {
                 f32x16 sc[KB] = {};
                 __builtin_amdgcn_s_setprio(1);
+                if (F32 && rough) {
+                    const float* f = (const float*)s_k + (r * HD + kept_here(h));
+#pragma unroll 4
+                    for (int d = 0; d < HD; d += 2) sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[d], (float)q[d + h] * sign, sc[0], 0, 0, 0);
+                } else {
 #pragma unroll
-                for (int d = 0; d < KK; d++)
+                    for (int d = 0; d < KK; d++)
 #pragma unroll
-                    for (int j = 0; j < KB; j++) {
-                        const int key = 32 * j + r;
-                        V8 kv[NP];
+                        for (int j = 0; j < KB; j++) {
+                            const int key = 32 * j + r;
+                            V8 kv[NP];
 #pragma unroll
-                        for (int p = 0; p < NP; p++) kv[p] = *(const V8*)&s_k[buf][p][key][((2 * d + h) ^ (key & (PC - 1))) * 8];
+                            for (int p = 0; p < NP; p++) kv[p] = *(const V8*)&s_k[buf][p][key][((2 * d + h) ^ (key & (PC - 1))) * 8];
 #pragma unroll
-                        for (int p = NP - 1; p >= 0; p--)  // the smallest products first
+                            for (int p = NP - 1; p >= 0; p--)  // the smallest products first
 #pragma unroll
-                            for (int p2 = NP - 1 - p; p2 >= 0; p2--) sc[j] = mfma32(kv[p], qv[p2][d], sc[j]);
-                    }
-                __builtin_amdgcn_s_setprio(0);
-                if (F32 && s_odd[t & 1][0] == t + 1) {
-                    // keys that are not finite: parts of zero would make NaN of them, so their scores come from the
-                    // rows themselves
-                    const int h4 = kept_here(4 * h);
-#pragma unroll
-                    for (int j = 0; j < KB; j++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = base + 32 * j + 8 * (i / 4) + h4 + i % 4;
-                            float x = 0.f, odd = 0.f;
-                            if (key < seen)
-#pragma unroll 1
-                                for (int d = 0; d < HD; d++) {
-                                    const float y = (float)kb[(int64_t)key * a.k_stride + d];
-                                    x += (float)q[d] * y;
-                                    odd = __builtin_fmaf(y, 0.f, odd);
-                                }
-                            if (odd != odd) sc[j][i] = x * sign;
+                                for (int p2 = NP - 1 - p; p2 >= 0; p2--) sc[j] = mfma32(kv[p], qv[p2][d], sc[j]);
                         }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (base + BN > wave_least) {
                     const int own = kept_here(seen - base - 4 * h);  // a branch, not selects in every tile
 #pragma unroll
@@ -316,7 +357,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
                         for (int i = 0; i < 16; i++)
                             if (32 * j + 8 * (i / 4) + i % 4 >= own) sc[j][i] = -__builtin_inff();
                 }
-                const float to_base2 = F32 ? __builtin_ldexpf(factor, -kshift) : c;
+                // kept from 0 and infinity, so that -inf times it stays what it is
+                const float to_base2 = !F32 || rough ? c : fminf(fmaxf(__builtin_ldexpf(factor, -kshift), 0x1p-126f), 0x1p127f);
                 float next = -__builtin_inff();
 #pragma unroll
                 for (int j = 0; j < KB; j++)
@@ -339,38 +381,47 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
                         sc[j][i] = exp2_hw(__builtin_fmaf(sc[j][i], to_base2, -lift));
                         l += sc[j][i];
                     }
+                if (F32 && rough) {
+                    const float* f = (const float*)s_v + (kept_here(4 * h) * HD + r);
 #pragma unroll
-                for (int j = 0; j < KB; j++)
+                    for (int i = 0; i < 16; i++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        V8 pv[NP];
-                        __builtin_amdgcn_s_setprio(1);
+                        for (int d = 0; d < DT; d++)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_ldexpf(f[(8 * (i / 4) + i % 4) * HD + 32 * d], vshift), sc[0][i], o[d], 0, 0, 0);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            E part[NP];
-                            split_finite(sc[j][8 * u + e], part);
+                    for (int j = 0; j < KB; j++)
 #pragma unroll
-                            for (int p = 0; p < NP; p++) pv[p][e] = part[p];
-                        }
-                        const int i = lane & 15, key = 32 * j + 16 * u + 4 * h + i / 4;
+                        for (int u = 0; u < 2; u++) {
+                            V8 pv[NP];
+                            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                        for (int d = 0; d < DT; d++) {
-                            const int piece = 4 * d + 2 * (lane >> 4 & 1) + (i >> 1 & 1);
-                            V8 vt[NP];
+                            for (int e = 0; e < 8; e++) {
+                                E part[NP];
+                                split_finite(sc[j][8 * u + e], part);
 #pragma unroll
-                            for (int p = 0; p < NP; p++) {
-                                const V4 lo = read_columns<V4>(&s_v[buf][p][key][(piece ^ (2 * key & (PC - 1))) * 8 + 4 * (i & 1)]);
-                                const V4 hi = read_columns<V4>(&s_v[buf][p][key + 8][(piece ^ (2 * (key + 8) & (PC - 1))) * 8 + 4 * (i & 1)]);
-                                vt[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                                for (int p = 0; p < NP; p++) pv[p][e] = part[p];
                             }
+                            const int i = lane & 15, key = 32 * j + 16 * u + 4 * h + i / 4;
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; p--)
+                            for (int d = 0; d < DT; d++) {
+                                const int piece = 4 * d + 2 * (lane >> 4 & 1) + (i >> 1 & 1);
+                                V8 vt[NP];
 #pragma unroll
-                                for (int p2 = NP - 1 - p; p2 >= 0; p2--) o[d] = mfma32(vt[p], pv[p2], o[d]);
+                                for (int p = 0; p < NP; p++) {
+                                    const V4 lo = read_columns<V4>(&s_v[buf][p][key][(piece ^ (2 * key & (PC - 1))) * 8 + 4 * (i & 1)]);
+                                    const V4 hi = read_columns<V4>(&s_v[buf][p][key + 8][(piece ^ (2 * (key + 8) & (PC - 1))) * 8 + 4 * (i & 1)]);
+                                    vt[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                                }
+#pragma unroll
+                                for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                                    for (int p2 = NP - 1 - p; p2 >= 0; p2--) o[d] = mfma32(vt[p], pv[p2], o[d]);
+                            }
                         }
-                    }
+                }
                 __builtin_amdgcn_s_setprio(0);
-                if (s_odd[t & 1][1] == t + 1) {
+                if (s_odd[t & 1] == t + 1) {
                     // what was left out of the values, to the rows that see it
                     const int h4 = kept_here(4 * h);
                     for (int key = base; key < base + BN; key++)

@@ -161,6 +161,27 @@ def test_large_and_infinite_scores(ctx):
     assert torch.isnan(nc.paged_attention(ctx, nc.PagedKV(cache.k, cache.v), b, q)).all()
 
 
+@pytest.mark.parametrize("qt,ct", TYPES, ids=ids)
+@pytest.mark.parametrize("what", ["inf", "nan", "largest", "lowest"])
+def test_later_rows_reach_no_earlier_one(ctx, qt, ct, what):
+    """What the later of a sequence's new rows hold, and the places behind its end, is not seen before them."""
+    lens, rows = [300, 37, 257], [5, 3, 2]
+    cache = _sequences(lens, 16, 2, 128, ct, 85)
+    q = _randn((10, 8, 128), 86, 1.5, qt)
+    info = torch.finfo(ct)
+    x = {"inf": math.inf, "nan": math.nan, "largest": info.max, "lowest": info.min}[what]
+    for s, n in enumerate(lens):
+        pg, at = cache.place(s, n - 1)
+        cache.k[pg, at], cache.v[pg, at] = x, x
+    out = nc.paged_attention(ctx, nc.PagedKV(cache.k, cache.v), nc.PagedBatch(cache.table, ints(lens), ints(starts(rows))), q)
+    a = starts(rows)
+    for s, (n, m) in enumerate(zip(rows, lens)):
+        k, v = cache.read(s, m - 1)
+        r = slice(int(a[s]), int(a[s + 1]) - 1)
+        want, tol = attend(q[r], k, v, 128**-0.5)
+        close(out[r], want, weights_rounded(tol, v, qt), (what, s))
+
+
 @pytest.mark.parametrize("ct", [F32, F16], ids=ids)
 def test_bad_pages_and_lengths_answer_nan(ctx, ct):
     lens = [40, 300, 64]
