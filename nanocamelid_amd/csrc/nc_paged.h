@@ -205,33 +205,23 @@ __device__ __forceinline__ float sum_across(float x) {
     return v[0] + v[1];
 }
 
-// The wave's largest of v.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    auto up = [&](auto dpp) {
-        const uint32_t x = __builtin_amdgcn_update_dpp(0, v, decltype(dpp)::value, 0xf, 0xf, false);
-        v = x > v ? x : v;
-    };
-    up(std::integral_constant<int, 0x111>());  // row_shr:1, 2, 4, 8, then row_bcast:15 and 31 (lanes without a
-    up(std::integral_constant<int, 0x112>());  // source see 0)
-    up(std::integral_constant<int, 0x114>());
-    up(std::integral_constant<int, 0x118>());
-    up(std::integral_constant<int, 0x142>());
-    up(std::integral_constant<int, 0x143>());
-    return __builtin_amdgcn_readlane(v, 63);
+// v or what DPP brings from another lane (0 where there is none), whichever is larger.
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+    const uint32_t x = __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+    return x > v ? x : v;
 }
-
-// The largest of v in each group of 8 or 16 lanes, in the group's last lane.
+// The largest of v in each group of 8 or 16 lanes, in the group's last lane (row_shr:1, 2, 4, 8).
 template <int LANES>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-    auto up = [&](auto dpp) {
-        const uint32_t x = __builtin_amdgcn_update_dpp(0, v, decltype(dpp)::value, 0xf, 0xf, false);
-        v = x > v ? x : v;
-    };
-    up(std::integral_constant<int, 0x111>());
-    up(std::integral_constant<int, 0x112>());
-    up(std::integral_constant<int, 0x114>());
-    if (LANES == 16) up(std::integral_constant<int, 0x118>());
-    return v;
+    v = max_dpp<0x114>(max_dpp<0x112>(max_dpp<0x111>(v)));
+    return LANES == 16 ? max_dpp<0x118>(v) : v;
+}
+// The largest of the groups' last lanes, in the wave's last lane (row_shr:8, then row_bcast:15 and 31).
+template <int LANES>
+__device__ __forceinline__ uint32_t wave_max_of_groups(uint32_t v) {
+    if (LANES == 8) v = max_dpp<0x118>(v);
+    return max_dpp<0x143>(max_dpp<0x142>(v));
 }
 
 // The sum of v over the lanes up to the own one: within rows of 16 lanes, then the rows' last ones onto the next.

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
         const A* vb = (const A*)a.v + (int64_t)kbegin * a.v_stride + kvh * HD;
 
         V8 qv[NP][KK];
-        float factor = c;  // of the row's scores, to base 2
+        int qshift = 0;  // f32: the row of queries is scaled by 2^qshift
         if constexpr (F32) {
             float x[KK][8], top = 0.f;
 #pragma unroll
@@ -140,14 +140,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
                 for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[d][e]));
             }
             top = max_across<32>(top);
-            const int shift = shift_of(__float_as_uint(top));
-            factor = __builtin_ldexpf(c, -shift);
+            qshift = shift_of(__float_as_uint(top));
 #pragma unroll
             for (int d = 0; d < KK; d++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     E part[NP];
-                    split_parts(__builtin_ldexpf(x[d][e] * sign, shift), part);
+                    split_parts(__builtin_ldexpf(x[d][e] * sign, qshift), part);
 #pragma unroll
                     for (int p = 0; p < NP; p++) qv[p][d][e] = part[p];
                 }
@@ -229,11 +228,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
                         vl = vm[i] != 0 && vm[i] < vl ? vm[i] : vl;
                     }
                 }
-                kt = wave_max(kt);
-                vt = wave_max(vt);
-                kl = ~wave_max(~kl);
-                vl = ~wave_max(~vl);
-                if (lane == 0) *(u32x4*)s_size[w] = u32x4{kt, vt, kl, vl};
+                // a smallest is the largest of the complements; both end in the wave's last lane
+                kt = wave_max_of_groups<PC>(kt);
+                vt = wave_max_of_groups<PC>(vt);
+                kl = ~wave_max_of_groups<PC>(~kl);
+                vl = ~wave_max_of_groups<PC>(~vl);
+                if (lane == 63) *(u32x4*)s_size[w] = u32x4{kt, vt, kl, vl};
             } else if ((t + 1) * BN > before + q0 + 1) {
                 float odd = 0.f;  // NaN if there is one
 #pragma unroll
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ?
                             if (32 * j + 8 * (i / 4) + i % 4 >= own) sc[j][i] = -__builtin_inff();
                 }
                 // kept from 0 and infinity, so that -inf times it stays what it is
-                const float to_base2 = !F32 || rough ? c : fminf(fmaxf(__builtin_ldexpf(factor, -kshift), 0x1p-126f), 0x1p127f);
+                const float to_base2 = !F32 || rough ? c : fminf(fmaxf(__builtin_ldexpf(c, -qshift - kshift), 0x1p-126f), 0x1p127f);
                 float next = -__builtin_inff();
 #pragma unroll
                 for (int j = 0; j < KB; j++)
@@ -507,7 +507,7 @@ extern "C" int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t 
     if (type == NC_TYPE_BF16) return head_dim == 64 ? launch.template operator()<__bf16, 64, 4>() : launch.template operator()<__bf16, 128, 4>();
     if (head_dim == 64) return launch.template operator()<float, 64, 4>();
     // Eight waves share the splitting of a tile, a third of a wave's vector work, as long as that does not take more
-    // than 64 rows of a sequence together (4096 rows, 32 heads over 8: 458 us with eight, 493 with four; six prompts
-    // of up to 1200 rows, 24 heads over 8: 216 and 207).
+    // than 64 rows of a sequence together (4096 rows, 32 heads over 8: 462 us with eight, 512 with four; six prompts
+    // of up to 1200 rows, 24 heads over 8: 232 and 218).
     return a.together == 4 ? launch.template operator()<float, 128, 8>() : launch.template operator()<float, 128, 4>();
 }

@@ -163,6 +163,15 @@ def test_f32_rows_of_unlike_size(ctx, heads, hd):
     _check(tiny, q * 1e-25, k * 1e-25, v, [200], [200], hd**-0.5)
 
 
+@pytest.mark.parametrize("heads,hd", [(2, 64), (4, 128)])
+@pytest.mark.parametrize("e", [-122, 122])
+def test_f32_ordinary_scores_of_sizes_at_the_ends(ctx, heads, hd, e):
+    q, k, v = (x.contiguous() for x in _fused(70, heads, 1, hd, 50, F32))
+    q, k = torch.ldexp(q, torch.tensor(e, device="cuda")), torch.ldexp(k, torch.tensor(-e, device="cuda"))
+    assert torch.isfinite(q).all() and torch.isfinite(k).all()
+    _check(nc.packed_attention(ctx, q, k, v, ints([0, 70])), q, k, v, [70], [70], hd**-0.5)
+
+
 def test_scale(ctx):
     q, k, v = _fused(90, 2, 2, 64, 51, F32)
     for scale in (1.0, 0.0, -0.2):
