@@ -224,6 +224,11 @@ __device__ __forceinline__ uint32_t wave_max_of_groups(uint32_t v) {
     return max_dpp<0x143>(max_dpp<0x142>(v));
 }
 
+// The wave's largest of v.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    return __builtin_amdgcn_readlane(wave_max_of_groups<16>(group_max<16>(v)), 63);
+}
+
 // The sum of v over the lanes up to the own one: within rows of 16 lanes, then the rows' last ones onto the next.
 __device__ __forceinline__ int wave_prefix_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
@@ -234,6 +239,8 @@ __device__ __forceinline__ int wave_prefix_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
     return v;
 }
+// The wave's sum of v.
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_prefix_sum(v), 63); }
 
 constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
