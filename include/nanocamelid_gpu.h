@@ -229,7 +229,8 @@ int nc_rope_table(int64_t positions, int32_t rope_dim, float freq_base, float fa
  * rope_dim / 2, turn by rope[position][j] (device f32, as nc_rope_table's), each product and sum
  * rounded to f32 by itself as in the sessions; rope NULL: no rotation.  The cache gets each value
  * rounded once to its type.  q_out and k_out (NULL: not wanted) receive the rotated rows,
- * contiguous, of `type`; they may be q and k themselves where those are contiguous.  A row of no
+ * contiguous, of `type`; they may be q and k themselves where those are contiguous, and overlap
+ * nothing else of the call.  A row of no
  * position is given back unrotated; one past rope_positions gives NaN in the rotated pairs and is
  * not appended. */
 int nc_paged_kv_append(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch* batch, int type, int64_t rows,
@@ -241,7 +242,10 @@ int nc_paged_kv_append(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch*
  * stride, out contiguous of `type`; type F32 or the cache's.  Any number of rows a sequence; meant
  * for one (decode) to some (verify).  Scores, maxima and sums are f32; a row whose every score is
  * -inf answers zeros.  A row's result depends on neither the batch nor the other rows of its
- * sequence.  work: device scratch of nc_paged_attention_work_bytes (0: may be NULL), 16-byte
+ * sequence, down to the bit.  Positions that a row does not see may hold anything, NaN too.  F32 rows
+ * over a cache of 16 bits are multiplied in parts, as exact as f32 products for finite ones; an
+ * infinity in a row or in a key that it sees may make the row NaN.  out overlaps neither q nor the
+ * pools.  work: device scratch of nc_paged_attention_work_bytes (0: may be NULL), 16-byte
  * aligned, used by this call alone until it has finished. */
 int64_t nc_paged_attention_work_bytes(const nc_paged_kv* kv, const nc_paged_batch* batch, int64_t rows, int32_t heads);
 int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch* batch, int type, int64_t rows,
@@ -253,7 +257,12 @@ int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch*
  * heads * head_dim], k and v [kv_rows][kv_heads * head_dim] of `type` (F32, F16, BF16) with row
  * strides in elements, 16-byte aligned; out contiguous of `type`.  Scores, maxima and sums are f32.
  * A row that sees no key answers zeros, and so does one whose every score is -inf; rows outside
- * every sequence are left as they were; starts outside the tensors count as their ends. */
+ * every sequence are left as they were; starts outside the tensors count as their ends.  Weights of
+ * F16 and BF16 rows are rounded to that type.  F32 products are of 16-bit parts: a score is off by some 2^-22
+ * of |q||k|, as sums of f32 are, and a value of any dimension by 2^-22 of itself or 2^-40 of the largest of its
+ * 32 keys, whichever is more; keys and values of very unlike size (2^16 times) in those 32 cost time, not
+ * accuracy.  Keys and values that a row does not see may hold anything; an infinity in a row or in a key that
+ * it sees may make the row NaN.  out overlaps none of q, k and v. */
 int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t kv_rows, const void* q, int64_t q_stride,
                         const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t heads,
                         int32_t kv_heads, int32_t head_dim, const int32_t* seq_start, const int32_t* kv_start,

@@ -216,6 +216,8 @@ def rope_table(positions: int, rope_dim: int, freq_base: float = 500000.0, scali
     """The sessions' (sin, cos) angles of positions 0 .. positions - 1, [positions][rope_dim / 2][2] f32
     (cached_rope_angles, src/inference.rs:860-901).  scaling: (factor, original_context_length,
     low_freq_factor, high_freq_factor) of the Llama-3 frequency scaling, or None.  Needs no GPU."""
+    if positions < 0 or rope_dim < 0:
+        _refuse("rope_table", "positions and rope_dim cannot be negative")
     out = np.empty((positions, rope_dim // 2, 2), np.float32)
     check(lib().nc_rope_table(positions, rope_dim, float(freq_base), *(float(x) for x in scaling or (0, 0, 0, 0)),
                               out.ctypes.data))
@@ -331,8 +333,9 @@ def paged_kv_append(ctx: Context, cache: PagedKV, batch: PagedBatch, k, v, rope=
     who = "paged_kv_append"
     _same_device(who, ctx, cache, batch)
     code = _element_type(who, k)
-    hd, dtype, device, rows = cache.head_dim, k.dtype, ctx.device, k.shape[0]
+    hd, dtype, device = cache.head_dim, k.dtype, ctx.device
     ks = _rows(who, "k", k, cache.kv_heads, hd, dtype, device, -1)
+    rows = k.shape[0]
     vs = _rows(who, "v", v, cache.kv_heads, hd, dtype, device, rows)
     qs, heads, qp, qo, ko = 0, 0, None, None, None
     if q is not None:
@@ -357,7 +360,8 @@ def paged_kv_append(ctx: Context, cache: PagedKV, batch: PagedBatch, k, v, rope=
 def paged_attention(ctx: Context, cache: PagedKV, batch: PagedBatch, q, scale: float | None = None, out=None):
     """Attention of the newest rows q [rows][heads][head_dim] of each sequence over its pages, up to each
     row's own position; query head h reads kv head h // (heads / kv_heads).  q is float32 or of the
-    cache's type; scale defaults to 1 / sqrt(head_dim).  Returns [rows][heads][head_dim] of q's type.  The
+    cache's type; scale defaults to 1 / sqrt(head_dim).  Returns [rows][heads][head_dim] of q's type, in out
+    if that is given, which overlaps neither q nor the pools.  The
     scratch comes from torch's allocator on the current stream, so calls on different streams, and captured
     graphs, share none."""
     import torch
@@ -386,7 +390,8 @@ def packed_attention(ctx: Context, q, k, v, seq_start, kv_start=None, scale: flo
     of one type (float32, float16, bfloat16), sequence s being the rows seq_start[s] .. seq_start[s + 1] (int32
     device tensor) and, where kv_start is given, the keys kv_start[s] .. kv_start[s + 1]: the last query row of
     a sequence sees all of its keys, the one before all but the last, and so on.  Rows may be views of a fused
-    buffer.  Returns [rows][heads][head_dim]; rows outside every sequence are left as they were in out."""
+    buffer.  Returns [rows][heads][head_dim], in out if that is given, which overlaps none of the others; rows
+    outside every sequence are left as they were in it.  Accuracy of float32: nanocamelid_gpu.h."""
     who = "packed_attention"
     code = _element_type(who, q)
     if q.dim() != 3 or k.dim() != 3 or seq_start.dim() != 1 or seq_start.shape[0] < 1:

@@ -500,6 +500,7 @@ extern "C" int nc_packed_attention(nc_ctx* ctx, int type, int64_t rows, int64_t 
             return fail(NC_EINVAL, "nc_packed_attention: rows must be 16-byte aligned and not overlap");
     if ((uintptr_t)out % 16 || (uintptr_t)seq_start % 4 || (uintptr_t)kv_start % 4)
         return fail(NC_EINVAL, "nc_packed_attention: misaligned output or starts");
+    if (out == q || out == k || out == v) return fail(NC_EINVAL, "nc_packed_attention: the output must not be one of the inputs");
     PackedParams a = {q, k, v, q_stride, k_stride, v_stride, out, seq_start, kv_start ? kv_start : seq_start, seqs,
                       (int32_t)rows, (int32_t)kv_rows, heads, kv_heads, 1, scale};
     DeviceGuard guard(ctx->device);

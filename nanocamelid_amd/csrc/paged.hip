@@ -141,7 +141,7 @@ __device__ __forceinline__ void lds_barrier() {
 //   f32: products of 16 x 16 x 4, whose operands need no turning.
 // A wave takes 32 or 64 positions at once: all their loads are in flight together, and one maximum serves them.
 template <typename A, typename C, int HD, int RT, bool ONE>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void paged_attention_kernel(PagedAttnParams a) {
+__global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attention_kernel(PagedAttnParams a) {
     constexpr bool F32 = sizeof(C) == 4;
     constexpr int KW = kWaveKeys<C, HD>, CH = 4 * KW, KT = KW / 16;
     constexpr bool BF = std::is_same_v<C, __bf16>;
@@ -758,7 +758,7 @@ int read_cache(const char* who, const nc_paged_kv* kv, const nc_paged_batch* b, 
 }
 
 bool bad_rows(const void* p, int64_t stride, int64_t width, int size) {
-    return (uintptr_t)p % 16 || stride < width || stride * size % 16;
+    return (uintptr_t)p % 16 || stride < width || stride > (INT64_MAX >> 34) || stride * size % 16;
 }
 
 // Calls f with the element types of the activations and the cache.
@@ -802,8 +802,8 @@ AttnPlan plan_attention(const nc_paged_kv& kv, const PagedSeqs& s, int heads) {
     const int64_t chunks = std::max<int64_t>(((int64_t)s.cap + p.chunk - 1) / p.chunk, 1);
     // From 8 units a CU on, the chip is full without a split along the positions, and two chunks are faster done in
     // turn than joined.  Otherwise a workgroup takes a chunk, or where there may be more of them than fit the chip
-    // at once (two workgroups a CU, one with two tiles) an equal part of all.
-    const int64_t units = kv.kv_heads * p.units, fit = p.tiles == 1 ? 512 : 256;
+    // at once (two workgroups a CU, one with two tiles of 128 dimensions) an equal part of all.
+    const int64_t units = kv.kv_heads * p.units, fit = p.tiles == 1 || kv.head_dim == 64 ? 512 : 256;
     if (chunks > 2 && units < 2048) {
         p.slots = (int)std::min<int64_t>(chunks, INT32_MAX);
         p.balanced = units * chunks > fit;
@@ -873,6 +873,7 @@ extern "C" int64_t nc_paged_attention_work_bytes(const nc_paged_kv* kv, const nc
     if (int rc = read_cache("nc_paged_attention_work_bytes", kv, batch, rows, s, p)) return rc;
     if (heads < 1 || heads % kv->kv_heads || kv->kv_heads > 65535)
         return fail(NC_EINVAL, "nc_paged_attention_work_bytes: heads must be a multiple of the cache's heads, those at most 65535");
+    if (rows * heads > INT32_MAX - 512) return fail(NC_ERANGE, "nc_paged_attention_work_bytes: too many rows and heads");
     const AttnPlan plan = plan_attention(*kv, s, heads);
     return plan.bytes(rows, heads, kv->head_dim);
 }
@@ -893,6 +894,7 @@ extern "C" int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_p
     if (!q || !out) return fail(NC_EINVAL, "nc_paged_attention: null argument");
     if (bad_rows(q, q_stride, (int64_t)heads * kv->head_dim, size) || (uintptr_t)out % 16)
         return fail(NC_EINVAL, "nc_paged_attention: rows must be 16-byte aligned and not overlap");
+    if (out == q) return fail(NC_EINVAL, "nc_paged_attention: the output must not be the queries");
     const AttnPlan plan = plan_attention(*kv, a.seqs, heads);
     a.units = plan.units;
     const int64_t need = plan.bytes(rows, heads, kv->head_dim);

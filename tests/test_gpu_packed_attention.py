@@ -240,10 +240,10 @@ def test_nothing_to_do(ctx):
     assert (out == 2).all()
 
 
-@pytest.mark.parametrize("what", ["mixed", "int", "heads", "head_dim", "rows", "start_type", "start_shape", "strided", "unaligned", "cpu", "out"])
+@pytest.mark.parametrize("what", ["mixed", "int", "heads", "head_dim", "rows", "start_type", "start_shape", "strided", "unaligned", "cpu", "out", "out_is_q", "out_is_k"])
 def test_refusals(ctx, what):
     q, k = _randn((8, 4, 64), 111), _randn((8, 2, 64), 112)
-    s = ints([0, 8])
+    s, q2 = ints([0, 8]), q.clone()
     calls = {
         "mixed": lambda: nc.packed_attention(ctx, q, k.half(), k, s),
         "int": lambda: nc.packed_attention(ctx, q.int(), k.int(), k.int(), s),
@@ -256,6 +256,8 @@ def test_refusals(ctx, what):
         "unaligned": lambda: nc.packed_attention(ctx, q, k, _randn((8, 129), 1)[:, 1:].view(8, 2, 64), s),
         "cpu": lambda: nc.packed_attention(ctx, q.cpu(), k.cpu(), k.cpu(), s.cpu()),
         "out": lambda: nc.packed_attention(ctx, q, k, k, s, out=torch.empty((8, 2, 64), device="cuda")),
+        "out_is_q": lambda: nc.packed_attention(ctx, q, k, k, s, out=q),
+        "out_is_k": lambda: nc.packed_attention(ctx, q, q2, q2, s, out=q2),
     }
     with pytest.raises(nc.NcError) as e:
         calls[what]()

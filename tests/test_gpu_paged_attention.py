@@ -467,7 +467,8 @@ def test_nothing_to_do(ctx):
 
 
 @pytest.mark.parametrize("what", ["type", "heads", "head_dim", "row_shape", "other_rows", "strided_heads", "unaligned", "rows_without_starts",
-                                  "pools_differ", "pool_inner_stride", "pool_type", "table_type", "cpu_rows", "rope_type", "rope_wide", "out_shape"])
+                                  "pools_differ", "pool_inner_stride", "pool_type", "table_type", "cpu_rows", "rope_type", "rope_wide", "out_is_q", "no_dimensions",
+                                  "out_shape"])
 def test_refusals(ctx, what):
     cache = _sequences([20, 20], 16, 2, 64, F16, 271)
     pool, batch = nc.PagedKV(cache.k, cache.v), nc.PagedBatch(cache.table, ints([20, 20]))
@@ -489,6 +490,8 @@ def test_refusals(ctx, what):
         "cpu_rows": lambda: nc.paged_attention(ctx, pool, batch, q.cpu()),
         "rope_type": lambda: nc.paged_kv_append(ctx, pool, batch, k, k, angles.double()),
         "rope_wide": lambda: nc.paged_kv_append(ctx, pool, batch, k, k, torch.from_numpy(nc.rope_table(20, 128)).cuda()),
+        "out_is_q": lambda: nc.paged_attention(ctx, pool, batch, q, out=q),
+        "no_dimensions": lambda: nc.paged_kv_append(ctx, pool, batch, k[0, 0, 0], k),
         "out_shape": lambda: nc.paged_attention(ctx, pool, batch, q, out=torch.empty((2, 4, 128), device="cuda")),
     }
     with pytest.raises(nc.NcError) as e:

@@ -136,14 +136,14 @@ def _append(kv=KV, batch=BATCH, **a):
 
 
 def _attend(kv=KV, batch=BATCH, **a):
-    a = {**dict(type=0, rows=5, q=ADDRESS, qs=256, heads=4, out=ADDRESS, work=ADDRESS, bytes=1 << 40), **a}
+    a = {**dict(type=0, rows=5, q=ADDRESS, qs=256, heads=4, out=2 * ADDRESS, work=ADDRESS, bytes=1 << 40), **a}
     return F.lib().nc_paged_attention(_ctx(), C.byref(F.PagedKVView(**kv)), C.byref(F.PagedBatchView(**batch)), a["type"], a["rows"], a["q"],
                                       a["qs"], a["heads"], 1.0, a["out"], a["work"], a["bytes"], None)
 
 
 def _packed(**a):
     a = {**dict(type=0, rows=5, kv_rows=5, q=ADDRESS, qs=256, k=ADDRESS, ks=128, v=ADDRESS, vs=128, heads=4, kv=2, hd=64, start=ADDRESS,
-                kv_start=None, seqs=2, out=ADDRESS), **a}
+                kv_start=None, seqs=2, out=2 * ADDRESS), **a}
     return F.lib().nc_packed_attention(_ctx(), a["type"], a["rows"], a["kv_rows"], a["q"], a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["heads"],
                                        a["kv"], a["hd"], a["start"], a["kv_start"], a["seqs"], 1.0, a["out"], None)
 
@@ -168,13 +168,13 @@ def test_bad_batches_are_refused(field, value):
 
 @pytest.mark.parametrize("args", [dict(type=2), dict(k=None), dict(v=None), dict(q_out=None), dict(heads=0), dict(ks=127), dict(ks=64), dict(vs=130),
                                   dict(k=ADDRESS + 4), dict(q=ADDRESS + 8), dict(qs=255), dict(k_out=ADDRESS + 4), dict(q_out=ADDRESS + 4), dict(dim=0),
-                                  dict(dim=63), dict(dim=128), dict(positions=0), dict(rope=ADDRESS + 2)])
+                                  dict(dim=63), dict(dim=128), dict(positions=0), dict(rope=ADDRESS + 2), dict(ks=1 << 40)])
 def test_bad_appends_are_refused(args):
     assert _append(**args) == F.NC_EINVAL
 
 
 @pytest.mark.parametrize("args", [dict(type=F.NC_TYPE_BF16), dict(type=99), dict(q=None), dict(out=None), dict(heads=5), dict(heads=0), dict(qs=128),
-                                  dict(q=ADDRESS + 4), dict(out=ADDRESS + 4)])
+                                  dict(q=ADDRESS + 4), dict(out=ADDRESS + 4), dict(out=ADDRESS), dict(qs=1 << 40)])
 def test_bad_attentions_are_refused(args):
     assert _attend(**args) == F.NC_EINVAL
 
@@ -183,13 +183,16 @@ def test_bad_attentions_are_refused(args):
                                        (dict(rows=-1), -5), (dict(kv_rows=1 << 31), -5), (dict(seqs=-1), -5), (dict(q=None), -1), (dict(k=None), -1),
                                        (dict(out=None), -1), (dict(start=None), -1), (dict(kv_rows=4), -1), (dict(ks=64), -1), (dict(vs=130), -1),
                                        (dict(q=ADDRESS + 4), -1), (dict(out=ADDRESS + 8), -1), (dict(start=ADDRESS + 2), -1),
-                                       (dict(qs=1 << 40), -1)])
+                                       (dict(qs=1 << 40), -1), (dict(out=ADDRESS), -1), (dict(q=3 * ADDRESS, out=ADDRESS), -1)])
 def test_bad_packed_attentions_are_refused(args, code):
     assert _packed(**args) == code
 
 
 def test_rows_beyond_an_index_are_refused():
     assert _append(rows=1 << 31) == F.NC_ERANGE and _attend(rows=-1) == F.NC_ERANGE
+    assert _attend(rows=1 << 30) == F.NC_ERANGE
+    batch = C.byref(F.PagedBatchView(**BATCH))
+    assert F.lib().nc_paged_attention_work_bytes(C.byref(F.PagedKVView(**KV)), batch, 1 << 30, 4) == F.NC_ERANGE
 
 
 def test_nothing_to_do_is_no_error():
