@@ -658,13 +658,34 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
 }
 
 // The chunks of one (row, head) by a wave, a few dimensions a lane.  The running maxima, which only compare, come
-// from a scan over the lanes, 64 chunks at a time, so that the chunks' loads do not wait for each other.
+// from a scan over the lanes, 64 chunks at a time, so that the chunks' loads do not wait for each other: 32 are in
+// flight while 32 are added.
+//
+// Bound by latency: few rows, and three loads after each other before a sum is known to count (59 chunks of 32 rows
+// 7 us, most of it the start and the loads), by the partial sums' bytes where rows are many (51 MB, 48 rows of 64
+// heads of up to 32 chunks: 11 us, 4.6 TB/s).
 template <typename A, int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams a, int chunk) {
     constexpr int ND = HD / 64;
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (unit >= (int64_t)a.seqs.rows * a.heads) return;
+    typedef float O __attribute__((ext_vector_type(ND)));
+    const float* ml = a.part_ml + unit * a.slots * 2;
+    const O* o = (const O*)(a.part_o + unit * a.slots * HD) + lane;
+    constexpr int B = 32;
+    O x[B], y[B];
+    // The first ones are asked for before their number is known: the row's slots are there, written or not
+    f32x2 mine = *(const f32x2*)(ml + 2 * (lane < a.slots ? lane : 0));
+    auto load = [&](O(&x)[B], int c0, int chunks, int from) {
+#pragma unroll
+        for (int i = from; i < B; i += 16)
+            if (c0 + i < chunks)
+#pragma unroll
+                for (int j = i; j < i + 16; j++) x[j] = o[(int64_t)(c0 + j < chunks ? c0 + j : chunks - 1) * (HD / ND)];
+    };
+#pragma unroll
+    for (int j = 0; j < 16; j++) x[j] = o[(int64_t)(j < a.slots ? j : a.slots - 1) * (HD / ND)];
     const int t = (int)(unit / a.heads);
     const int s = seq_of_row(a.seqs.row_start, a.seqs.seqs, t);
     if (s < 0) return;
@@ -675,20 +696,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams a, int 
     const int seen = (int)(seen64 < 0 ? 0 : seen64 > a.seqs.cap ? a.seqs.cap : seen64);
     const int chunks = seen > 0 ? (seen - 1) / chunk + 1 : 1;
     if (chunks == 1) return;  // answered already
-    typedef float O __attribute__((ext_vector_type(ND)));
-    const float* ml = a.part_ml + unit * a.slots * 2;
-    const O* o = (const O*)(a.part_o + unit * a.slots * HD) + lane;
+    load(x, 0, chunks, 16);
     RowSum<ND> sum;
     if (seen64 > a.seqs.cap) sum.l = __builtin_nanf("");
     for (int c0 = 0; c0 < chunks; c0 += 64) {
-        const int c = c0 + lane, count = chunks - c0 < 64 ? chunks - c0 : 64;
-        O x[64];
-#pragma unroll
-        for (int i = 0; i < 64; i += 16)
-            if (i < count)
-#pragma unroll
-                for (int j = i; j < i + 16; j++) x[j] = o[(int64_t)(c0 + (j < count ? j : count - 1)) * (HD / ND)];
-        const f32x2 mine = c < chunks ? *(const f32x2*)(ml + 2 * c) : f32x2{-__builtin_inff(), 0.f};
+        if (c0 + lane >= chunks) mine = f32x2{-__builtin_inff(), 0.f};
         float top = fmaxf(mine[0], sum.m);  // the largest score up to this chunk
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -697,17 +709,23 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams a, int 
         }
         float prev = __shfl_up(top, 1, 64);
         if (lane == 0) prev = sum.m;
-        const float base = exp_base(top), f = exp2_hw(prev - base), g = exp2_hw(mine[0] - base);
+        const float base = exp_base(top), f = exp2_hw(prev - base), g = exp2_hw(mine[0] - base), l2 = mine[1];
+        sum.m = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), 63));
+        if (c0 + 64 < chunks) mine = *(const f32x2*)(ml + 2 * (c0 + 64 + lane < chunks ? c0 + 64 + lane : chunks - 1));
         auto of = [](float v, int at) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), at)); };
+        for (int b = 0; b < 64 && c0 + b < chunks; b += B) {
+            load(y, c0 + b + B, chunks, 0);
 #pragma unroll
-        for (int j = 0; j < 64; j++)
-            if (j < count) {
-                float y[ND];
+            for (int j = 0; j < B; j++)
+                if (c0 + b + j < chunks) {
+                    float z[ND];
 #pragma unroll
-                for (int d = 0; d < ND; d++) y[d] = x[j][d];
-                sum.add(0.f, of(mine[1], j), of(f, j), of(g, j), y);
-            }
-        sum.m = of(top, 63);
+                    for (int d = 0; d < ND; d++) z[d] = x[j][d];
+                    sum.add(sum.m, of(l2, b + j), of(f, b + j), of(g, b + j), z);
+                }
+#pragma unroll
+            for (int j = 0; j < B; j++) x[j] = y[j];
+        }
     }
     A* out = (A*)a.out + unit * HD + ND * lane;
 #pragma unroll
