@@ -150,9 +150,10 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
     constexpr bool QSCALE = QP == 2;                           // f16 parts: the row scaled into f16's range
     // f16 weights carry 2^14, which keeps small ones normal numbers and cancels in the answer
     constexpr float PSHIFT = !F32 && !BF ? 14.f : 0.f;
-    // The next chunk's keys and values beside this one's, where the registers hold them; otherwise each half of the
-    // values takes the place of that half of the keys, and the next chunk's keys theirs.
-    constexpr bool EARLY = RT == 1 && (F32 || HD == 64 || ONE);
+    // A single chunk's keys and values are asked for at once.  Otherwise each half of the values takes the place of that
+    // half of the keys, and the next chunk's keys theirs: the next chunk's beside this one's, where registers allow,
+    // were slower (24 rows of up to 4000 positions, 64 dimensions, f32: 50 us against 45, bf16: 29 and 27).
+    constexpr bool EARLY = RT == 1 && ONE;
     constexpr int JB = RT == 1 && QP < 3 && !ONE ? 2 : 1;  // LDS buffers of the waves' joining
     constexpr int OS = HD + 4;     // LDS row, skewed by four banks
     constexpr int ND = HD / 16;    // dimensions of a thread in the chunk's sum
@@ -294,10 +295,10 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
             const int all_chunks = most > 0 ? (most - 1) / CH + 1 : 1, chunks = all_chunks < c_to ? all_chunks : c_to;
             if (c >= chunks) continue;
 
-            // A wave's keys and values of a chunk.  Each is loaded as soon as the chunk before no longer needs its
-            // registers: keys when their scores are done, values when they are summed, so that loads are in flight
-            // through the softmax and the waves' joining.  They are issued whether or not there is a next chunk: behind
-            // a branch, every wait for an earlier load would have to wait for these as well.
+            // A wave's keys and values of a chunk.  Values are asked for as the scores of their keys are done, the next
+            // chunk's keys as the values are summed, so that loads are in flight through the softmax and the waves'
+            // joining.  They are issued whether or not there is a next chunk: behind a branch, every wait for an earlier
+            // load would have to wait for these as well.
             typedef uint32_t VL __attribute__((ext_vector_type(F32 ? 4 : HD / 32)));  // 16 bytes, or HD / 16 values
             constexpr int KV = QV, NV = F32 ? HD / 64 : 1;
             u32x4 kx[KT][KV];
@@ -457,10 +458,6 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
                         publish(buf ^ 1, next);
                         ask(next + step);
                     }
-                    if (!ONE && EARLY) {
-#pragma unroll
-                        for (int half = 0; half < 2; half++) load_keys(buf ^ 1, half);
-                    }
 #pragma unroll
                     for (int t = 0; t < RT; t++) {
                         const float factor = s_factor[t][r];
@@ -545,7 +542,7 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
 #pragma unroll
                                         for (int t = 0; t < RT; t++)
                                             o[t][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vx[j][i][h][e]), sc[t][j][i], o[t][4 * h + e], 0, 0, 0);
-                            if (!ONE && !EARLY && j % (KT / 2) == KT / 2 - 1) load_keys(buf ^ 1, 2 * j / KT);
+                            if (!ONE && j % (KT / 2) == KT / 2 - 1) load_keys(buf ^ 1, 2 * j / KT);
                         }
                     } else {
 #pragma unroll
@@ -574,7 +571,7 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
 #pragma unroll
                                     for (int p = PP - 1; p >= 0; p--) o[t][e] = mfma16(vt, pv[t][p], o[t][e]);
                             }
-                            if (!ONE && !EARLY && b % (KT / 4) == KT / 4 - 1) load_keys(buf ^ 1, 4 * b / KT);
+                            if (!ONE && b % (KT / 4) == KT / 4 - 1) load_keys(buf ^ 1, 4 * b / KT);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -596,10 +593,6 @@ __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attent
                                             if (base + key < seen[t]) o[t][e][i] += v;
                                 }
                         }
-                    }
-                    if (!ONE && EARLY) {
-#pragma unroll
-                        for (int half = 0; half < 2; half++) load_values(buf ^ 1, half);
                     }
                 }
                 buf ^= 1;
@@ -811,21 +804,27 @@ AttnPlan plan_attention(const nc_paged_kv& kv, const PagedSeqs& s, int heads) {
     AttnPlan p;
     const int64_t group = heads / kv.kv_heads, seqs = std::max(s.seqs, 1);
     p.chunk = kv.head_dim == 128 && kv.elem_type == NC_TYPE_F32 ? 128 : 256;
-    // Two tiles where sequences may have more than 16 rows (of the average, or twice that where they differ): one
-    // tile would read their keys and values twice.
+    // Two tiles where sequences have more than 16 rows: with one, their keys and values are read twice.  Where they
+    // may differ, from an average of 25 on (16 sequences of up to 3000 positions in f32, 4 query heads a kv head: of
+    // up to 5 new rows, 10 on average, 62 us with one and 68 with two; up to 8: 65 and 70; up to 16: 109 and 97).
     const int64_t rows = ((int64_t)s.rows + seqs - 1) / seqs * group;
-    p.tiles = (s.row_start ? 2 * rows : rows) <= 16 ? 1 : 2;
+    p.tiles = rows <= (s.row_start ? 24 : 16) ? 1 : 2;
     const int64_t high = 16 * p.tiles;
     p.units = s.row_start ? (int64_t)s.rows * group / high + seqs : seqs * ((group + high - 1) / high);
     const int64_t chunks = std::max<int64_t>(((int64_t)s.cap + p.chunk - 1) / p.chunk, 1);
-    // From 8 units a CU on, the chip is full without a split along the positions, and two chunks are faster done in
-    // turn than joined.  Otherwise a workgroup takes a chunk, or where there may be more of them than fit the chip
-    // at once (two workgroups a CU, one with two tiles of 128 dimensions) an equal part of all.
+    // A workgroup takes a chunk, or where there may be more of them than fit the chip at once (two workgroups a CU, one
+    // with two tiles of 128 dimensions) an equal part of all, and the chunks are joined afterwards.  A join costs some
+    // 7 us, as much as three chunks in turn (8 kv heads, 128 dimensions of 16 bits, chunks of 256; joined and in
+    // turn: one row of 700 positions 13.5 and 14.1 us, of 1000 14 and 17, of 15000 23 and 163), and parts
+    // stream slower than workgroups that stay with a unit: they are for units that leave CUs idle or of very
+    // different lengths (24 rows of up to 2000 positions 33 and 30 us, 40 of up to 3000 62 and 70, 48 of up to 8000
+    // 208 and 218; 64 of up to 600, 2000 and 8000 31 and 22, 69 and 70, 235 and 240; 128 of up to 4000 228 and 209).
     const int64_t units = kv.kv_heads * p.units, fit = p.tiles == 1 || kv.head_dim == 64 ? 512 : 256;
-    if (chunks > 2 && units < 2048) {
+    const bool fits = units * chunks <= fit;
+    if (fits ? chunks > 3 : chunks > 8 && units < fit * 3 / 2) {
         p.slots = (int)std::min<int64_t>(chunks, INT32_MAX);
-        p.balanced = units * chunks > fit;
-        p.along = (int)(p.balanced ? std::max<int64_t>(fit / kv.kv_heads, 1) * kv.kv_heads : chunks);
+        p.balanced = !fits;
+        p.along = (int)(fits ? chunks : std::max<int64_t>(fit / kv.kv_heads, 1) * kv.kv_heads);
     }
     p.one = p.along == chunks && !p.balanced;
     return p;

@@ -235,6 +235,21 @@ def test_a_rows_result_depends_on_no_other_row(ctx, qt, ct):
     assert torch.equal(again, step)
 
 
+@pytest.mark.parametrize("qt,ct,heads,kv,hd,seqs,most,rows", [
+    (F32, F32, 32, 8, 128, 12, 1400, 1), (F16, F16, 8, 2, 64, 40, 2600, 1), (F32, BF16, 4, 4, 128, 24, 2400, 1),
+    (F32, F32, 8, 1, 128, 20, 1400, 5), (BF16, BF16, 16, 2, 64, 30, 2500, 3), (F32, F16, 12, 1, 128, 8, 9000, 4), (F32, F32, 2, 1, 128, 300, 1200, 1)], ids=ids)
+def test_long_ragged_batches(ctx, qt, ct, heads, kv, hd, seqs, most, rows):
+    """More chunks than workgroups: each takes a part of all of them, which begins and ends within sequences.  The
+    answers are those of each sequence by itself."""
+    lens = [most] + [max(rows, most * (s * 7 % 23) // (23 if s % 3 else 230)) for s in range(1, seqs)]
+    cache = _sequences(lens, 16, kv, hd, ct, 121)
+    q, _, out = _check(ctx, cache, lens, [rows] * seqs, heads, kv, hd, qt, 122)
+    for s in {0, 1, seqs // 2, seqs - 1}:
+        own = nc.PagedBatch(cache.table[s:s + 1], ints([lens[s]]), ints([0, rows]))
+        alone = nc.paged_attention(ctx, nc.PagedKV(cache.k, cache.v), own, q[s * rows:(s + 1) * rows])
+        assert torch.equal(alone, out[s * rows:(s + 1) * rows]), s
+
+
 @pytest.mark.parametrize("ct", [F16, F32], ids=ids)
 def test_offsets_past_32_bits(ctx, ct):
     """Pools of more than 2^31 elements, the sequence's pages at their end."""
