@@ -65,6 +65,11 @@ __device__ __forceinline__ V4 read_columns(const void* p) {
 //   scores' factor and the answer give back.  The f32 products of the matrix cores run at a sixteenth of the f16
 //   rate, these at a third.  Where keys or values of a tile differ in size by more (a huge one that only later rows
 //   see, say), or one is not finite, the tile takes the f32 products.
+//
+// Measured, 32 heads over 8: 8192 rows of 128 dimensions in bf16 630 to 646 us, 850 to 870 TFLOP/s (a large product
+// 1039); 4096 rows in f32 462 us, 297 TFLOP/s, of three times as many f16 ones (with f32 products 1159 us, at 118;
+// their peak rate would need 938); 24 prompts of up to 700 rows of 64 dimensions in f16 47 us, 350 TFLOP/s: half the
+// dimensions have half the products for the same softmax.  A fourth wave a SIMD, of 128 registers, spills: 110 us.
 template <typename A, int HD, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : HD == 64 && sizeof(A) == 2 ? 3 : 2) void packed_attention_kernel(PackedParams a, int64_t units) {
     constexpr bool F32 = sizeof(A) == 4;

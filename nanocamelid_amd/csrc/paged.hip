@@ -32,7 +32,8 @@ struct AppendParams {
 // Bound by bytes: every value is read and written once.  A thread moves eight values of one row (16 or 32
 // bytes each way); their loads go out before the row's place is known, which takes three dependent loads
 // (its sequence, the length, the page).  A workgroup takes 256 of a row's units, so a decode batch still
-// spreads over many CUs.
+// spreads over many CUs.  Four prompts of up to 2711 rows, 32 heads over 8 of 128 dimensions, f32 into f16: 244 MB
+// in 40 us, 6.1 TB/s, 53 us a call where calls follow each other; 48 sequences of up to 5 rows 5 us, one row 3 us.
 template <typename A, typename C, int HD>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams a) {
     constexpr int U = HD / 8;  // units of a head
@@ -140,6 +141,12 @@ __device__ __forceinline__ void lds_barrier() {
 //   Weights of 16-bit rows are two parts as well: one alone would round as much as the answer's own rounding.
 //   f32: products of 16 x 16 x 4, whose operands need no turning.
 // A wave takes 32 or 64 positions at once: all their loads are in flight together, and one maximum serves them.
+//
+// Measured: 48 rows of 64 heads over 8 of 128 dimensions, bf16, up to 8000 positions: 870 MB in 197 us, 4.4 TB/s (a
+// kernel that reads without a table reaches 6.3, a copy 4.8); 16 sequences of up to 5 rows, f32, up to 3000
+// positions: 227 MB in 47 us, 4.8 TB/s; one row over 15000 positions in f16: 61 MB in 15 us.  The bytes fetched are
+// the cache's own.  What is lost is lost between chunks, where four waves join and the table's next pages are looked
+// up; loads that bypass the caches, 32 positions of 16 bits a wave and keys read in the values' pattern were no faster.
 template <typename A, typename C, int HD, int RT, bool ONE>
 __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attention_kernel(PagedAttnParams a) {
     constexpr bool F32 = sizeof(C) == 4;
