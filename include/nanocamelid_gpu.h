@@ -245,8 +245,9 @@ int nc_paged_kv_append(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch*
  * sequence, down to the bit.  Positions that a row does not see may hold anything, NaN too.  F32 rows
  * over a cache of 16 bits are multiplied in parts, as exact as f32 products for finite ones; an
  * infinity in a row or in a key that it sees may make the row NaN.  out overlaps neither q nor the
- * pools.  work: device scratch of nc_paged_attention_work_bytes (0: may be NULL), 16-byte
- * aligned, used by this call alone until it has finished. */
+ * pools.  work: device scratch of nc_paged_attention_work_bytes (asked for the same shape: it is not
+ * always more for more rows or positions; 0: may be NULL), 16-byte aligned, used by this call alone
+ * until it has finished. */
 int64_t nc_paged_attention_work_bytes(const nc_paged_kv* kv, const nc_paged_batch* batch, int64_t rows, int32_t heads);
 int nc_paged_attention(nc_ctx* ctx, const nc_paged_kv* kv, const nc_paged_batch* batch, int type, int64_t rows,
                        const void* q, int64_t q_stride, int32_t heads, float scale, void* out, void* work,

@@ -825,10 +825,12 @@ AttnPlan plan_attention(const nc_paged_kv& kv, const PagedSeqs& s, int heads) {
     // turn: one row of 700 positions 13.5 and 14.1 us, of 1000 14 and 17, of 15000 23 and 163), and parts
     // stream slower than workgroups that stay with a unit: they are for units that leave CUs idle or of very
     // different lengths (24 rows of up to 2000 positions 33 and 30 us, 40 of up to 3000 62 and 70, 48 of up to 8000
-    // 208 and 218; 64 of up to 600, 2000 and 8000 31 and 22, 69 and 70, 235 and 240; 128 of up to 4000 228 and 209).
+    // 208 and 218; 64 of up to 600, 2000 and 8000 31 and 22, 69 and 70, 235 and 240; 128 of up to 4000 228 and 209).  From 65
+    // chunks on they guard more units too against a long sequence among short ones, whose chunks take 2.8 us each in
+    // turn, at a cost where lengths are evenly spread (128 rows of up to 16000: 922 and 831 us).
     const int64_t units = kv.kv_heads * p.units, fit = p.tiles == 1 || kv.head_dim == 64 ? 512 : 256;
     const bool fits = units * chunks <= fit;
-    if (fits ? chunks > 3 : chunks > 8 && units < fit * 3 / 2) {
+    if (fits ? chunks > 3 : chunks > 8 && (units < fit * 3 / 2 || (chunks > 64 && units < 2048))) {
         p.slots = (int)std::min<int64_t>(chunks, INT32_MAX);
         p.balanced = !fits;
         p.along = (int)(fits ? chunks : std::max<int64_t>(fit / kv.kv_heads, 1) * kv.kv_heads);

@@ -250,6 +250,12 @@ def test_long_ragged_batches(ctx, qt, ct, heads, kv, hd, seqs, most, rows):
         assert torch.equal(alone, out[s * rows:(s + 1) * rows]), s
 
 
+def test_one_long_sequence_among_many(ctx):
+    lens = [1 + s * 13 % 60 for s in range(150)] + [17000] + [1 + s * 7 % 40 for s in range(59)]
+    cache = _sequences(lens, 16, 4, 64, F16, 125)
+    _check(ctx, cache, lens, [1] * len(lens), 8, 4, 64, F16, 126, row_start=False)
+
+
 @pytest.mark.parametrize("ct", [F16, F32], ids=ids)
 def test_offsets_past_32_bits(ctx, ct):
     """Pools of more than 2^31 elements, the sequence's pages at their end."""
