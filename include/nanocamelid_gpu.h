@@ -209,7 +209,7 @@ typedef struct nc_paged_kv {
  * padded batch) is not appended and answers zeros; rows outside every sequence are left as they
  * were; a row that needs a position past the table or max_len, or a page that is none of the pool's,
  * is not appended and answers NaN.  Pages may be shared by sequences that only read them; two rows
- * of one call that are appended to the same place leave either there. */
+ * of one call that are appended to the same place leave values of either there. */
 typedef struct nc_paged_batch {
     uint64_t table, lens, row_start; /* device int32 [seqs][table_stride], [seqs], [seqs + 1] or 0 */
     int64_t table_stride;            /* entries between rows of the table, at least table_pages */
