@@ -144,9 +144,10 @@ __device__ __forceinline__ void lds_barrier() {
 //
 // Measured: 48 rows of 64 heads over 8 of 128 dimensions, bf16, up to 8000 positions: 870 MB in 197 us, 4.4 TB/s (a
 // kernel that reads without a table reaches 6.3, a copy 4.8); 16 sequences of up to 5 rows, f32, up to 3000
-// positions: 227 MB in 47 us, 4.8 TB/s; one row over 15000 positions in f16: 61 MB in 15 us.  The bytes fetched are
-// the cache's own.  What is lost is lost between chunks, where four waves join and the table's next pages are looked
-// up; loads that bypass the caches, 32 positions of 16 bits a wave and keys read in the values' pattern were no faster.
+// positions: 227 MB in 47 us, 4.8 TB/s; one row over 15000 positions in f16: 61 MB in 15 us.  What is lost is lost
+// between chunks, where four waves join and the table's next pages are looked up: no byte of the cache is fetched
+// twice.  Loads that bypass the caches, 32 positions of 16 bits a wave and keys read in the values' pattern were no
+// faster.
 template <typename A, typename C, int HD, int RT, bool ONE>
 __global__ __launch_bounds__(256, RT == 1 || HD == 64 ? 2 : 1) void paged_attention_kernel(PagedAttnParams a) {
     constexpr bool F32 = sizeof(C) == 4;
