@@ -208,6 +208,24 @@ def test_bad_pages_and_lengths_answer_nan(ctx, ct):
     assert torch.isfinite(out[0]).all() and torch.isnan(out[1]).all() and torch.isfinite(out[2]).all()
 
 
+@pytest.mark.parametrize("seqs", [1, 40])
+@pytest.mark.parametrize("ct", [F16, F32], ids=ids)
+def test_bad_pages_and_lengths_of_joined_rows(ctx, ct, seqs):
+    lens = [2500] + [2450 - 60 * s for s in range(1, seqs)]
+    cache = _sequences(lens, 16, 2, 64, ct, 95)
+    q = _randn((3 * seqs, 4, 64), 96)
+    pool, at = nc.PagedKV(cache.k, cache.v), ints([3 * s for s in range(seqs + 1)])
+    good = nc.paged_attention(ctx, pool, nc.PagedBatch(cache.table, ints(lens), at), q)
+    assert torch.isfinite(good).all()
+    short = nc.paged_attention(ctx, pool, nc.PagedBatch(cache.table, ints(lens), at, max_len=2498), q)
+    assert torch.equal(short[:1], good[:1]) and torch.isnan(short[1:3]).all() and torch.equal(short[3:], good[3:])
+    table = cache.table.clone()
+    table[0, 2496 // 16] = cache.k.shape[0]  # the page of positions 2496 on: rows at 2497, 2498 and 2499 see it
+    table[0, 2500 // 16 + 1:] = -1           # pages that none sees
+    bad = nc.paged_attention(ctx, pool, nc.PagedBatch(table, ints(lens), at), q)
+    assert torch.isnan(bad[:3]).all() and torch.equal(bad[3:], good[3:])
+
+
 def test_row_starts_of_any_value_stay_inside(ctx):
     cache = _sequences([40, 50, 60], 16, 2, 64, F32, 101)
     q = _randn((8, 4, 64), 102)
@@ -456,6 +474,36 @@ def test_captured_step_follows_its_inputs(ctx):
         torch.cuda.synchronize()
         for _, out in graphs:
             assert torch.equal(out, eager), i
+
+
+@pytest.mark.parametrize("seqs", [2, 40])
+def test_captured_joins_have_scratch_of_their_own(ctx, seqs):
+    """Attention that is split and joined, in two graphs, replayed over lengths that change the chunks in use."""
+    heads, kv, hd, most = 8, 2, 64, 2600
+    lens_ = [most] + [1 + most * (s * 11 % 17) // 40 for s in range(1, seqs)]
+    cache = _sequences(lens_, 16, kv, hd, F16, 215)
+    pool, lens, q = nc.PagedKV(cache.k, cache.v), ints(lens_), _randn((seqs, heads, hd), 216)
+    batch = nc.PagedBatch(cache.table, lens)
+    assert nc.lib().nc_paged_attention_work_bytes(pool.ref, batch.ref, seqs, heads) > 0
+    qs = [q, _randn((seqs, heads, hd), 217)]
+    nc.paged_attention(ctx, pool, batch, q)
+    torch.cuda.synchronize()
+    graphs = []
+    for x in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = nc.paged_attention(ctx, pool, batch, x)
+        graphs.append((graph, out))
+    for i in range(4):
+        lens.copy_(ints([max(1, n - 700 * i) for n in lens_]))
+        q.copy_(_randn((seqs, heads, hd), 218 + i))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = [nc.paged_attention(ctx, pool, batch, x) for x in qs]
+        torch.cuda.synchronize()
+        for (_, out), want in zip(graphs, eager):
+            assert torch.equal(out, want), i
 
 
 def test_two_streams_at_once(ctx):
